@@ -40,6 +40,7 @@ extern "C" {
 #define LSB_DTYPE_F32 0
 #define LSB_DTYPE_BF16 1
 #define LSB_DTYPE_F16 2
+#define LSB_DTYPE_E4M3 3 /* quantised KV caches only (lsb_paged_attn kv_dtype) */
 
 /* Attention forward implementation selector (lsb_attn_fwd `impl`). */
 #define LSB_IMPL_AUTO 0    /* tcgen05 kernel when eligible, else SIMT kernel */
@@ -227,6 +228,84 @@ LSB_API int lsb_rope_kv_write_slots(const void* qkv, int64_t s_s, int64_t s_part
                                     void* q_out, void* k_out, void* k_cache, void* v_cache,
                                     int64_t T, int64_t H, int64_t D, int64_t num_blocks,
                                     int64_t block_size, int dtype, void* stream);
+
+/*
+ * Quantised paged KV cache. New operators: lightserve leaves the cache's layout
+ * to the deployment (engine/config.py:7-11). K and V are e4m3
+ * [num_blocks, H, block_size, D] and k_scale / v_scale e8m0 [num_blocks, H,
+ * block_size], one scale per (token, head): a value is e4m3 * 2^(scale - 127),
+ * the scale being the smallest that takes the row's largest finite magnitude
+ * to 448 or less (1 at least). NaN and infinities are stored as e4m3's NaN.
+ *
+ * lsb_kv_quantize: lsb_kv_cache_write into such a cache. k, v: [T, H, D]
+ * (strides {t, h} in elements, d contiguous); slots outside the cache are
+ * skipped; the others must differ.
+ * lsb_kv_dequantize: k_out, v_out [T, H, D] contiguous of `dtype` from the
+ * rows at slot_mapping (zeros for slots outside the cache; results past
+ * dtype's largest finite value are held there).
+ */
+LSB_API int lsb_kv_quantize(const void* k, const void* v, void* k_cache, void* v_cache,
+                            void* k_scale, void* v_scale, const int64_t* slot_mapping, int64_t T,
+                            int64_t H, int64_t D, int64_t num_blocks, int64_t block_size,
+                            int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h, int dtype,
+                            void* stream);
+LSB_API int lsb_kv_dequantize(const void* k_cache, const void* v_cache, const void* k_scale,
+                              const void* v_scale, const int64_t* slot_mapping, void* k_out,
+                              void* v_out, int64_t T, int64_t H, int64_t D, int64_t num_blocks,
+                              int64_t block_size, int dtype, void* stream);
+
+/*
+ * lsb_rope_kv_write and lsb_rope_kv_write_slots into a quantised cache, with
+ * their roundings: exactly one of slot_mapping (int64 [T]) and block_tables
+ * (int32 [T, max_blocks_per_seq], one token per sequence) is given. cos / sin
+ * have max_pos rows; a position outside them gives NaN in q_out and k_out,
+ * context length 0 and no cache write. k_out and context_lens may be NULL.
+ */
+LSB_API int lsb_rope_kv_quantize(const void* qkv, int64_t s_s, int64_t s_part, int64_t s_h,
+                                 const void* cos_table, const void* sin_table, int64_t s_pos,
+                                 int64_t max_pos, const int64_t* positions,
+                                 const int64_t* slot_mapping, const int32_t* block_tables,
+                                 int64_t max_blocks_per_seq, void* q_out, void* k_out,
+                                 void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                                 int32_t* context_lens, int64_t T, int64_t H, int64_t D,
+                                 int64_t num_blocks, int64_t block_size, int dtype, void* stream);
+
+/*
+ * Attention of new tokens over a paged KV cache (chunked prefill, prompts
+ * behind a cached prefix, drafted tokens, and decode with a window, shared
+ * heads or a quantised cache). New operator: engine/request.py:86-93 names the
+ * case, no kernel of lightserve serves it.
+ * q, o: [total_q, Hq, D] (strides {t, h}, d contiguous); the new tokens of
+ * sequence s are rows [cu_seqlens_q[s], cu_seqlens_q[s + 1]) (int32
+ * [num_seqs + 1]; NULL: one row per sequence), max_seqlen_q at most; they are
+ * the last of its context_lens[s] cached tokens. k_cache, v_cache:
+ * [num_blocks, Hkv, block_size, D] contiguous, of kv_dtype: `dtype`, or
+ * LSB_DTYPE_E4M3 with k_scale / v_scale. Query head h reads cache head
+ * h / (Hq / Hkv). The row at position p sees key j when j <= p,
+ * j < context_lens[s], j's block id lies in [0, num_blocks) and, when
+ * window > 0, p - j < window or j < num_sinks. A row that sees none gives 0.
+ * lse (optional): fp32 [Hq, total_q], natural log (-inf when no key is seen).
+ * Rows of no sequence, or past max_seqlen_q of theirs, are left as they were.
+ * workspace: >= lsb_paged_attn_workspace_size bytes, 16-byte aligned (may be
+ * NULL when that size is 0); calls that run at the same time need their own.
+ * impl: LSB_IMPL_AUTO, or one of the kernels (error when it does not serve
+ * the call).
+ */
+LSB_API int64_t lsb_paged_attn_workspace_size(int64_t num_seqs, int64_t total_q,
+                                              int64_t max_seqlen_q, int64_t Hq, int64_t Hkv,
+                                              int64_t D, int64_t max_blocks_per_seq,
+                                              int64_t block_size, int64_t window,
+                                              int64_t num_sinks);
+LSB_API int lsb_paged_attn(const void* q, const void* k_cache, const void* v_cache,
+                           const void* k_scale, const void* v_scale,
+                           const int32_t* block_tables, const int32_t* context_lens,
+                           const int32_t* cu_seqlens_q, void* o, float* lse, int64_t num_seqs,
+                           int64_t total_q, int64_t max_seqlen_q, int64_t Hq, int64_t Hkv,
+                           int64_t D, int64_t max_blocks_per_seq, int64_t block_size,
+                           int64_t num_blocks, int64_t sq_t, int64_t sq_h, int64_t so_t,
+                           int64_t so_h, int64_t window, int64_t num_sinks, float scale,
+                           int dtype, int kv_dtype, int impl, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 /*
  * Fused SwiGLU of the Llama MLP: out = silu(gate) * up with

@@ -26,6 +26,7 @@ LSB_ERR_CUDA = 3
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
+DTYPE_E4M3 = 3  # quantised KV caches only
 
 IMPL_AUTO = 0
 IMPL_SIMT = 1
@@ -64,6 +65,12 @@ SIGNATURES = {
                                _I64, _I64, _I64, _I64, _I64, _I, _P]),
     "lsb_rope_kv_write_slots": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _P, _P,
                                      _I64, _I64, _I64, _I64, _I64, _I, _P]),
+    "lsb_kv_quantize": (_I, [_P] * 7 + [_I64] * 9 + [_I, _P]),
+    "lsb_kv_dequantize": (_I, [_P] * 7 + [_I64] * 5 + [_I, _P]),
+    "lsb_rope_kv_quantize": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _I64,
+                                  _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I, _P]),
+    "lsb_paged_attn_workspace_size": (_I64, [_I64] * 10),
+    "lsb_paged_attn": (_I, [_P] * 10 + [_I64] * 15 + [_F, _I, _I, _I, _P, _I64, _P]),
     "lsb_swiglu": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I, _P]),
     "lsb_greedy_next": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
     "lsb_linear_packed_bytes": (_I64, [_I64, _I64]),

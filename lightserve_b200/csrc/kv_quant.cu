@@ -1,0 +1,513 @@
+// Quantised paged KV cache: writing rows, writing rows with the rotary
+// embedding fused in, and reading rows back (all HBM-bound).
+//
+// Layout, per layer: K and V as e4m3 [num_blocks, H, block_size, D] and their
+// scales as e8m0 [num_blocks, H, block_size] (fp8.cuh has the format), so the
+// block tables and slots of the 16-bit cache address it unchanged.
+//
+// Vectorised kernels: LPR = D * sizeof(T) / 16 lanes hold one row of K, V or
+// q as one 16-byte vector each, so a warp's loads are whole contiguous
+// sectors; the row's maximum is a butterfly over those lanes, and a lane's 8
+// (16-bit types) or 4 (fp32) bytes make the row's 32- to 256-byte run in the
+// cache. The rotary partner x[i +- D/2] sits LPR / 2 lanes away and comes by
+// shuffle. Any other head dim or alignment takes the warp-per-row kernels.
+#include "common.cuh"
+#include "fp8.cuh"
+
+#include <type_traits>
+
+namespace lsb {
+namespace kvq {
+
+constexpr int THREADS = 256;
+
+// Where one token's rows go: its cache slot, or -1 for none.
+struct SlotOf {
+  const int64_t* slots;          // [T] block * bs + offset, or NULL
+  const int64_t* positions;      // with block tables
+  const int32_t* block_tables;   // [T, max_blocks]
+  int64_t max_blocks;
+  int64_t num_blocks;
+  int bs;
+  __device__ __forceinline__ int64_t operator()(int64_t t) const {
+    if (slots != nullptr) {
+      const int64_t s = slots[t];
+      return s >= 0 && s < num_blocks * bs ? s : -1;
+    }
+    const int64_t pos = positions[t];
+    if (pos < 0 || pos / bs >= max_blocks) return -1;
+    const int64_t blk = block_tables[t * max_blocks + pos / bs];
+    return blk >= 0 && blk < num_blocks ? blk * bs + pos % bs : -1;
+  }
+};
+
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Quantises the row whose LANES lanes hold `f`, writing VEC bytes per lane
+// and the scale byte. Every lane of the warp takes part; `write` is false for
+// rows that have no slot.
+template <int LANES, int VEC>
+__device__ __forceinline__ void store_row(const float (&f)[VEC], bool write, int lane_in_row,
+                                          uint8_t* __restrict__ row, uint8_t* __restrict__ scale) {
+  float amax = 0.f;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) amax = fmaxf(amax, finite_abs(f[e]));
+  const int e8 = e8m0_of_amax(lanes_max<LANES>(amax));
+  const float inv = e8m0_inverse(e8);
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4; ++i)
+    w[i] = cvt_e4m3x2(scaled_for_e4m3(f[4 * i], inv), scaled_for_e4m3(f[4 * i + 1], inv)) |
+           (cvt_e4m3x2(scaled_for_e4m3(f[4 * i + 2], inv), scaled_for_e4m3(f[4 * i + 3], inv)) << 16);
+  if (!write) return;
+  if constexpr (VEC == 8)
+    *reinterpret_cast<uint2*>(row + lane_in_row * VEC) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(row + lane_in_row * VEC) = w[0];
+  if (lane_in_row == 0) *scale = (uint8_t)e8;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS)
+quantize_vec_kernel(const T* __restrict__ k, const T* __restrict__ v, uint8_t* __restrict__ k_cache,
+                    uint8_t* __restrict__ v_cache, uint8_t* __restrict__ k_scale,
+                    uint8_t* __restrict__ v_scale, const SlotOf slot_of, uint32_t rows, uint32_t H,
+                    int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h) {
+  allow_dependents();
+  wait_prerequisites();
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr int LPR = D / VEC;
+  const uint64_t g = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
+  const bool in = g / LPR < rows;
+  const uint32_t row = in ? (uint32_t)(g / LPR) : rows - 1;  // lanes past the end repeat the last row
+  const int c = (int)(g % LPR);
+  const uint32_t t = row / H, h = row % H;
+  const Vec16<T> kx = ld_vec16_stream(k + t * sk_t + h * sk_h + c * VEC);
+  const Vec16<T> vx = ld_vec16_stream(v + t * sv_t + h * sv_h + c * VEC);
+  const int64_t slot = slot_of(t);
+  const bool write = in && slot >= 0;
+  const int64_t cell = write ? ((slot / slot_of.bs) * H + h) * slot_of.bs + slot % slot_of.bs : 0;
+  float f[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] = to_f(kx.v[e]);
+  store_row<LPR>(f, write, c, k_cache + cell * D, k_scale + cell);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] = to_f(vx.v[e]);
+  store_row<LPR>(f, write, c, v_cache + cell * D, v_scale + cell);
+}
+
+// One warp per (token, head) row, any head dim and alignment. WITH_ROPE: see
+// rope_quantize_vec_kernel.
+template <typename T>
+__device__ __forceinline__ void store_row_any(const T* __restrict__ x, int D, uint8_t* __restrict__ row,
+                                              uint8_t* __restrict__ scale) {
+  const int lane = threadIdx.x & 31;
+  float amax = 0.f;
+  for (int d = lane; d < D; d += 32) amax = fmaxf(amax, finite_abs(to_f(x[d])));
+  const int e8 = e8m0_of_amax(warp_max(amax));
+  const float inv = e8m0_inverse(e8);
+  for (int d = lane; d < D; d += 32)
+    row[d] = (uint8_t)cvt_e4m3x2(scaled_for_e4m3(to_f(x[d]), inv), 0.f);
+  if (lane == 0) *scale = (uint8_t)e8;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+quantize_any_kernel(const T* __restrict__ k, const T* __restrict__ v, uint8_t* __restrict__ k_cache,
+                    uint8_t* __restrict__ v_cache, uint8_t* __restrict__ k_scale,
+                    uint8_t* __restrict__ v_scale, const SlotOf slot_of, uint32_t rows, uint32_t H,
+                    int D, int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h) {
+  allow_dependents();
+  wait_prerequisites();
+  const uint64_t row = ((uint64_t)blockIdx.x * THREADS + threadIdx.x) >> 5;
+  if (row >= rows) return;
+  const uint32_t t = (uint32_t)row / H, h = (uint32_t)row % H;
+  const int64_t slot = slot_of(t);
+  if (slot < 0) return;
+  const int64_t cell = ((slot / slot_of.bs) * H + h) * slot_of.bs + slot % slot_of.bs;
+  store_row_any(k + t * sk_t + h * sk_h, D, k_cache + cell * D, k_scale + cell);
+  store_row_any(v + t * sv_t + h * sv_h, D, v_cache + cell * D, v_scale + cell);
+}
+
+// ------------------------------------------------------------ read back ---
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS)
+dequantize_vec_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
+                      const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
+                      const SlotOf slot_of, T* __restrict__ k_out, T* __restrict__ v_out,
+                      uint32_t rows, uint32_t H) {
+  allow_dependents();
+  wait_prerequisites();
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr int LPR = D / VEC;
+  const uint64_t g = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
+  if (g / LPR >= rows) return;
+  const uint32_t row = (uint32_t)(g / LPR);
+  const int c = (int)(g % LPR);
+  const uint32_t t = row / H, h = row % H;
+  const int64_t slot = slot_of(t);
+  Vec16<T> ko, vo;
+  if (slot < 0) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) ko.v[e] = vo.v[e] = from_f<T>(0.f);
+  } else {
+    const int64_t cell = ((slot / slot_of.bs) * H + h) * slot_of.bs + slot % slot_of.bs;
+    const float ks = e8m0_to_float(k_scale[cell]), vs = e8m0_to_float(v_scale[cell]);
+    uint32_t kw[VEC / 4], vw[VEC / 4];
+    if constexpr (VEC == 8) {
+      const uint2 a = *reinterpret_cast<const uint2*>(k_cache + cell * D + c * VEC);
+      const uint2 b = *reinterpret_cast<const uint2*>(v_cache + cell * D + c * VEC);
+      kw[0] = a.x; kw[1] = a.y; vw[0] = b.x; vw[1] = b.y;
+    } else {
+      kw[0] = *reinterpret_cast<const uint32_t*>(k_cache + cell * D + c * VEC);
+      vw[0] = *reinterpret_cast<const uint32_t*>(v_cache + cell * D + c * VEC);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      float a[4], b[4];
+      e4m3x4_to_float(kw[i], a);
+      e4m3x4_to_float(vw[i], b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        ko.v[4 * i + e] = from_f<T>(clamp_finite<T>(a[e] * ks));
+        vo.v[4 * i + e] = from_f<T>(clamp_finite<T>(b[e] * vs));
+      }
+    }
+  }
+  const int64_t o = (int64_t)row * D + c * VEC;
+  __stcs(reinterpret_cast<uint4*>(k_out + o), *reinterpret_cast<const uint4*>(&ko));
+  __stcs(reinterpret_cast<uint4*>(v_out + o), *reinterpret_cast<const uint4*>(&vo));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+dequantize_any_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache,
+                      const uint8_t* __restrict__ k_scale, const uint8_t* __restrict__ v_scale,
+                      const SlotOf slot_of, T* __restrict__ k_out, T* __restrict__ v_out,
+                      uint32_t rows, uint32_t H, int D) {
+  allow_dependents();
+  wait_prerequisites();
+  const uint64_t row = ((uint64_t)blockIdx.x * THREADS + threadIdx.x) >> 5;
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  const uint32_t t = (uint32_t)row / H, h = (uint32_t)row % H;
+  const int64_t slot = slot_of(t);
+  const int64_t cell =
+      slot < 0 ? 0 : ((slot / slot_of.bs) * H + h) * slot_of.bs + slot % slot_of.bs;
+  const float ks = slot < 0 ? 0.f : e8m0_to_float(k_scale[cell]);
+  const float vs = slot < 0 ? 0.f : e8m0_to_float(v_scale[cell]);
+  for (int d = lane; d < D; d += 32) {
+    float a = 0.f, b = 0.f;
+    if (slot >= 0) {
+      a = f16x2_to_float2(cvt_e4m3x2_f16x2(k_cache[cell * D + d])).x * ks;
+      b = f16x2_to_float2(cvt_e4m3x2_f16x2(v_cache[cell * D + d])).x * vs;
+    }
+    k_out[(int64_t)row * D + d] = from_f<T>(clamp_finite<T>(a));
+    v_out[(int64_t)row * D + d] = from_f<T>(clamp_finite<T>(b));
+  }
+}
+
+// ------------------------------------------------- rotary + quantisation ---
+// rotate_half(x) = [-x2, x1]; each product and the sum rounded to T, as the
+// 16-bit cache's rotary write does, so q and the k that is quantised equal
+// its q and k bit for bit.
+template <typename T>
+__device__ __forceinline__ T rope1(float x, float turned, float c, float s) {
+  const float a = to_f(from_f<T>(__fmul_rn(x, c)));
+  const float b = to_f(from_f<T>(__fmul_rn(turned, s)));
+  return from_f<T>(__fadd_rn(a, b));
+}
+
+struct RopeArgs {
+  int64_t s_s, s_part, s_h;  // qkv strides
+  int64_t s_pos, max_pos;    // cos / sin row stride and rows
+  const int64_t* positions;
+  int32_t* context_lens;     // may be NULL
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS)
+rope_quantize_vec_kernel(const T* __restrict__ qkv, const T* __restrict__ cos_t,
+                         const T* __restrict__ sin_t, const RopeArgs a, T* __restrict__ q_out,
+                         T* __restrict__ k_out, uint8_t* __restrict__ k_cache,
+                         uint8_t* __restrict__ v_cache, uint8_t* __restrict__ k_scale,
+                         uint8_t* __restrict__ v_scale, const SlotOf slot_of, uint32_t rows,
+                         uint32_t H) {
+  allow_dependents();
+  wait_prerequisites();
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr int LPR = D / VEC;
+  static_assert(LPR >= 2 && LPR <= 32, "a row and its rotary partner live in one warp");
+  const uint64_t g = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
+  const bool in = g / LPR < rows;
+  const uint32_t row = in ? (uint32_t)(g / LPR) : rows - 1;
+  const int c = (int)(g % LPR);
+  const uint32_t t = row / H, h = row % H;
+  const T* x = qkv + t * a.s_s + h * a.s_h + c * VEC;
+  const Vec16<T> qx = ld_vec16_stream(x), kx = ld_vec16_stream(x + a.s_part),
+                 vx = ld_vec16_stream(x + 2 * a.s_part);
+  const int64_t pos = a.positions[t];
+  // A position outside the table has no angle: q (and k_out) become NaN and
+  // nothing is cached.
+  const bool known = pos >= 0 && pos < a.max_pos;
+  const Vec16<T> cx = ld_vec16(cos_t + (known ? pos : 0) * a.s_pos + c * VEC);
+  const Vec16<T> sx = ld_vec16(sin_t + (known ? pos : 0) * a.s_pos + c * VEC);
+  const int64_t slot = known ? slot_of(t) : -1;
+  if (in && h == 0 && c == 0 && a.context_lens != nullptr)
+    a.context_lens[t] = known ? (int32_t)(pos + 1) : 0;
+  const bool write = in && slot >= 0;
+  const int64_t cell = write ? ((slot / slot_of.bs) * H + h) * slot_of.bs + slot % slot_of.bs : 0;
+  const float sign = c < LPR / 2 ? -1.f : 1.f;  // first half takes -x2, second x1
+  auto turn = [&](const Vec16<T>& v, float (&f)[VEC], Vec16<T>& out) {
+    Vec16<T> p;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(&v);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(&p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = __shfl_xor_sync(0xffffffffu, src[i], LPR / 2);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const T r = rope1<T>(to_f(v.v[e]), sign * to_f(p.v[e]), to_f(cx.v[e]), to_f(sx.v[e]));
+      out.v[e] = known ? r : from_f<T>(__int_as_float(0x7fc00000));
+      f[e] = to_f(out.v[e]);
+    }
+  };
+  float f[VEC];
+  Vec16<T> o;
+  turn(qx, f, o);
+  if (in) st_vec16(q_out + (int64_t)row * D + c * VEC, o);
+  turn(kx, f, o);
+  if (in && k_out != nullptr) st_vec16(k_out + (int64_t)row * D + c * VEC, o);
+  store_row<LPR>(f, write, c, k_cache + cell * D, k_scale + cell);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) f[e] = to_f(vx.v[e]);
+  store_row<LPR>(f, write, c, v_cache + cell * D, v_scale + cell);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+rope_quantize_any_kernel(const T* __restrict__ qkv, const T* __restrict__ cos_t,
+                         const T* __restrict__ sin_t, const RopeArgs a, T* __restrict__ q_out,
+                         T* __restrict__ k_out, uint8_t* __restrict__ k_cache,
+                         uint8_t* __restrict__ v_cache, uint8_t* __restrict__ k_scale,
+                         uint8_t* __restrict__ v_scale, const SlotOf slot_of, uint32_t rows,
+                         uint32_t H, int D) {
+  allow_dependents();
+  wait_prerequisites();
+  const uint64_t row = ((uint64_t)blockIdx.x * THREADS + threadIdx.x) >> 5;
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31, half = D / 2;
+  const uint32_t t = (uint32_t)row / H, h = (uint32_t)row % H;
+  const int64_t pos = a.positions[t];
+  const bool known = pos >= 0 && pos < a.max_pos;
+  const T* cs = cos_t + (known ? pos : 0) * a.s_pos;
+  const T* sn = sin_t + (known ? pos : 0) * a.s_pos;
+  const int64_t slot = known ? slot_of(t) : -1;
+  if (h == 0 && lane == 0 && a.context_lens != nullptr)
+    a.context_lens[t] = known ? (int32_t)(pos + 1) : 0;
+  const T* q = qkv + t * a.s_s + h * a.s_h;
+  auto turned = [&](const T* x, int d) -> T {
+    if (!known) return from_f<T>(__int_as_float(0x7fc00000));
+    const float p = d < half ? -to_f(x[d + half]) : to_f(x[d - half]);
+    return rope1<T>(to_f(x[d]), p, to_f(cs[d]), to_f(sn[d]));
+  };
+  float amax = 0.f;
+  for (int d = lane; d < D; d += 32) {
+    q_out[(int64_t)row * D + d] = turned(q, d);
+    const T kr = turned(q + a.s_part, d);
+    if (k_out != nullptr) k_out[(int64_t)row * D + d] = kr;
+    amax = fmaxf(amax, finite_abs(to_f(kr)));
+  }
+  if (slot < 0) return;
+  const int64_t cell = ((slot / slot_of.bs) * H + h) * slot_of.bs + slot % slot_of.bs;
+  const int e8 = e8m0_of_amax(warp_max(amax));
+  const float inv = e8m0_inverse(e8);
+  for (int d = lane; d < D; d += 32)  // the rotation again, instead of D registers
+    k_cache[cell * D + d] =
+        (uint8_t)cvt_e4m3x2(scaled_for_e4m3(to_f(turned(q + a.s_part, d)), inv), 0.f);
+  if (lane == 0) k_scale[cell] = (uint8_t)e8;
+  store_row_any(q + 2 * a.s_part, D, v_cache + cell * D, v_scale + cell);
+}
+
+// Blocks for `rows` rows of `lanes` lanes each; 0 when the grid cannot hold them.
+static unsigned blocks_for(int64_t rows, int lanes) {
+  const int64_t b = (rows * lanes + THREADS - 1) / THREADS;
+  return b <= 0x7fffffff ? (unsigned)b : 0;
+}
+
+// Calls f(head dim constant) for the head dims the vectorised kernels serve.
+template <typename T, class F>
+static int with_dim(int64_t D, F&& f) {
+  if (D == 64) return f(std::integral_constant<int, 64>{});
+  if (D == 128) return f(std::integral_constant<int, 128>{});
+  if constexpr (sizeof(T) == 2) {
+    if (D == 256) return f(std::integral_constant<int, 256>{});
+  } else {
+    if (D == 32) return f(std::integral_constant<int, 32>{});
+  }
+  return -1;
+}
+
+static bool strides16(int esz, std::initializer_list<int64_t> s) {
+  for (int64_t x : s)
+    if ((x * esz) % 16 != 0) return false;
+  return true;
+}
+
+static bool aligned(std::initializer_list<const void*> p, uintptr_t to) {
+  for (const void* x : p)
+    if ((reinterpret_cast<uintptr_t>(x) & (to - 1)) != 0) return false;
+  return true;
+}
+
+static int check_sizes(const char* who, int64_t T, int64_t H, int64_t D, int64_t num_blocks,
+                       int64_t block_size, int dtype) {
+  LSB_CHECK_ARG(T >= 0 && H > 0 && D > 0 && num_blocks > 0 && block_size > 0,
+                "%s: bad sizes T=%lld H=%lld D=%lld num_blocks=%lld block_size=%lld", who,
+                (long long)T, (long long)H, (long long)D, (long long)num_blocks,
+                (long long)block_size);
+  LSB_CHECK_ARG(dtype_size(dtype) > 0, "%s: unsupported dtype %d", who, dtype);
+  LSB_CHECK_ARG(D <= 65536 && block_size <= 0x7fffffff && num_blocks <= 0x7fffffff &&
+                    H <= 0x7fffffff && T <= 0x7fffffff && T * H <= 0x7fffffff,
+                "%s: sizes too large (T * H is limited to 2^31 - 1)", who);
+  return LSB_OK;
+}
+
+}  // namespace kvq
+}  // namespace lsb
+
+extern "C" int lsb_kv_quantize(const void* k, const void* v, void* k_cache, void* v_cache,
+                               void* k_scale, void* v_scale, const int64_t* slot_mapping, int64_t T,
+                               int64_t H, int64_t D, int64_t num_blocks, int64_t block_size,
+                               int64_t sk_t, int64_t sk_h, int64_t sv_t, int64_t sv_h, int dtype,
+                               void* stream) {
+  using namespace lsb::kvq;
+  if (int rc = check_sizes("kv_quantize", T, H, D, num_blocks, block_size, dtype)) return rc;
+  if (T == 0) return LSB_OK;
+  LSB_CHECK_ARG(k && v && k_cache && v_cache && k_scale && v_scale && slot_mapping,
+                "kv_quantize: null pointer");
+  const SlotOf slot_of{slot_mapping, nullptr, nullptr, 0, num_blocks, (int)block_size};
+  const uint32_t rows = (uint32_t)(T * H);
+  cudaStream_t st = (cudaStream_t)stream;
+  return LSB_DISPATCH_DTYPE(dtype, Tt, [&] {
+    const bool vec = aligned({k, v}, 16) && aligned({k_cache, v_cache}, 8) &&
+                     strides16(sizeof(Tt), {sk_t, sk_h, sv_t, sv_h});
+    const int rc = vec ? with_dim<Tt>(D, [&](auto dim) -> int {
+      constexpr int DD = decltype(dim)::value;
+      const unsigned blocks = blocks_for(rows, DD * (int)sizeof(Tt) / 16);
+      LSB_CHECK_ARG(blocks > 0, "kv_quantize: too many rows");
+      LSB_CUDA_OK(lsb::launch_kernel(quantize_vec_kernel<Tt, DD>, dim3(blocks), dim3(THREADS), 0, st,
+                                     (const Tt*)k, (const Tt*)v, (uint8_t*)k_cache,
+                                     (uint8_t*)v_cache, (uint8_t*)k_scale, (uint8_t*)v_scale,
+                                     slot_of, rows, (uint32_t)H, sk_t, sk_h, sv_t, sv_h),
+                  "kv_quantize");
+      return LSB_OK;
+    }) : -1;
+    if (rc >= 0) return rc;
+    const unsigned blocks = blocks_for(rows, 32);
+    LSB_CHECK_ARG(blocks > 0, "kv_quantize: too many rows");
+    LSB_CUDA_OK(lsb::launch_kernel(quantize_any_kernel<Tt>, dim3(blocks), dim3(THREADS), 0, st,
+                                   (const Tt*)k, (const Tt*)v, (uint8_t*)k_cache, (uint8_t*)v_cache,
+                                   (uint8_t*)k_scale, (uint8_t*)v_scale, slot_of, rows, (uint32_t)H,
+                                   (int)D, sk_t, sk_h, sv_t, sv_h),
+                "kv_quantize");
+    return LSB_OK;
+  });
+}
+
+extern "C" int lsb_kv_dequantize(const void* k_cache, const void* v_cache, const void* k_scale,
+                                 const void* v_scale, const int64_t* slot_mapping, void* k_out,
+                                 void* v_out, int64_t T, int64_t H, int64_t D, int64_t num_blocks,
+                                 int64_t block_size, int dtype, void* stream) {
+  using namespace lsb::kvq;
+  if (int rc = check_sizes("kv_dequantize", T, H, D, num_blocks, block_size, dtype)) return rc;
+  if (T == 0) return LSB_OK;
+  LSB_CHECK_ARG(k_cache && v_cache && k_scale && v_scale && slot_mapping && k_out && v_out,
+                "kv_dequantize: null pointer");
+  const SlotOf slot_of{slot_mapping, nullptr, nullptr, 0, num_blocks, (int)block_size};
+  const uint32_t rows = (uint32_t)(T * H);
+  cudaStream_t st = (cudaStream_t)stream;
+  return LSB_DISPATCH_DTYPE(dtype, Tt, [&] {
+    const bool vec = aligned({k_out, v_out}, 16) && aligned({k_cache, v_cache}, 8);
+    const int rc = vec ? with_dim<Tt>(D, [&](auto dim) -> int {
+      constexpr int DD = decltype(dim)::value;
+      const unsigned blocks = blocks_for(rows, DD * (int)sizeof(Tt) / 16);
+      LSB_CHECK_ARG(blocks > 0, "kv_dequantize: too many rows");
+      LSB_CUDA_OK(lsb::launch_kernel(dequantize_vec_kernel<Tt, DD>, dim3(blocks), dim3(THREADS), 0,
+                                     st, (const uint8_t*)k_cache, (const uint8_t*)v_cache,
+                                     (const uint8_t*)k_scale, (const uint8_t*)v_scale, slot_of,
+                                     (Tt*)k_out, (Tt*)v_out, rows, (uint32_t)H),
+                  "kv_dequantize");
+      return LSB_OK;
+    }) : -1;
+    if (rc >= 0) return rc;
+    const unsigned blocks = blocks_for(rows, 32);
+    LSB_CHECK_ARG(blocks > 0, "kv_dequantize: too many rows");
+    LSB_CUDA_OK(lsb::launch_kernel(dequantize_any_kernel<Tt>, dim3(blocks), dim3(THREADS), 0, st,
+                                   (const uint8_t*)k_cache, (const uint8_t*)v_cache,
+                                   (const uint8_t*)k_scale, (const uint8_t*)v_scale, slot_of,
+                                   (Tt*)k_out, (Tt*)v_out, rows, (uint32_t)H, (int)D),
+                "kv_dequantize");
+    return LSB_OK;
+  });
+}
+
+extern "C" int lsb_rope_kv_quantize(const void* qkv, int64_t s_s, int64_t s_part, int64_t s_h,
+                                    const void* cos_table, const void* sin_table, int64_t s_pos,
+                                    int64_t max_pos, const int64_t* positions,
+                                    const int64_t* slot_mapping, const int32_t* block_tables,
+                                    int64_t max_blocks_per_seq, void* q_out, void* k_out,
+                                    void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                                    int32_t* context_lens, int64_t T, int64_t H, int64_t D,
+                                    int64_t num_blocks, int64_t block_size, int dtype,
+                                    void* stream) {
+  using namespace lsb::kvq;
+  if (int rc = check_sizes("rope_kv_quantize", T, H, D, num_blocks, block_size, dtype)) return rc;
+  LSB_CHECK_ARG(D % 2 == 0 && max_pos > 0, "rope_kv_quantize: D=%lld must be even, max_pos=%lld positive",
+                (long long)D, (long long)max_pos);
+  LSB_CHECK_ARG((slot_mapping == nullptr) != (block_tables == nullptr) || T == 0,
+                "rope_kv_quantize: give slot_mapping or block_tables, not both");
+  LSB_CHECK_ARG(block_tables == nullptr || max_blocks_per_seq > 0,
+                "rope_kv_quantize: max_blocks_per_seq=%lld must be positive",
+                (long long)max_blocks_per_seq);
+  if (T == 0) return LSB_OK;
+  LSB_CHECK_ARG(qkv && cos_table && sin_table && positions && q_out && k_cache && v_cache &&
+                    k_scale && v_scale,
+                "rope_kv_quantize: null pointer");
+  const SlotOf slot_of{slot_mapping, positions, block_tables, max_blocks_per_seq, num_blocks,
+                       (int)block_size};
+  const RopeArgs args{s_s, s_part, s_h, s_pos, max_pos, positions, context_lens};
+  const uint32_t rows = (uint32_t)(T * H);
+  cudaStream_t st = (cudaStream_t)stream;
+  return LSB_DISPATCH_DTYPE(dtype, Tt, [&] {
+    const bool vec = aligned({qkv, cos_table, sin_table, q_out, k_out}, 16) &&
+                     aligned({k_cache, v_cache}, 8) &&
+                     strides16(sizeof(Tt), {s_s, s_part, s_h, s_pos});
+    const int rc = vec ? with_dim<Tt>(D, [&](auto dim) -> int {
+      constexpr int DD = decltype(dim)::value;
+      const unsigned blocks = blocks_for(rows, DD * (int)sizeof(Tt) / 16);
+      LSB_CHECK_ARG(blocks > 0, "rope_kv_quantize: too many rows");
+      LSB_CUDA_OK(lsb::launch_kernel(rope_quantize_vec_kernel<Tt, DD>, dim3(blocks), dim3(THREADS),
+                                     0, st, (const Tt*)qkv, (const Tt*)cos_table,
+                                     (const Tt*)sin_table, args, (Tt*)q_out, (Tt*)k_out,
+                                     (uint8_t*)k_cache, (uint8_t*)v_cache, (uint8_t*)k_scale,
+                                     (uint8_t*)v_scale, slot_of, rows, (uint32_t)H),
+                  "rope_kv_quantize");
+      return LSB_OK;
+    }) : -1;
+    if (rc >= 0) return rc;
+    const unsigned blocks = blocks_for(rows, 32);
+    LSB_CHECK_ARG(blocks > 0, "rope_kv_quantize: too many rows");
+    LSB_CUDA_OK(lsb::launch_kernel(rope_quantize_any_kernel<Tt>, dim3(blocks), dim3(THREADS), 0, st,
+                                   (const Tt*)qkv, (const Tt*)cos_table, (const Tt*)sin_table, args,
+                                   (Tt*)q_out, (Tt*)k_out, (uint8_t*)k_cache, (uint8_t*)v_cache,
+                                   (uint8_t*)k_scale, (uint8_t*)v_scale, slot_of, rows, (uint32_t)H,
+                                   (int)D),
+                "rope_kv_quantize");
+    return LSB_OK;
+  });
+}

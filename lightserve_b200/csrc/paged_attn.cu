@@ -1,0 +1,426 @@
+// Attention of new tokens over a paged KV cache: the C entry, the choice of
+// kernel, the CUDA-core kernel (any type, head dim up to 256, any alignment)
+// and the kernel that joins split key ranges. paged_attn.cuh has the
+// definitions.
+#include "paged_attn.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace lsb {
+namespace pa {
+
+// ------------------------------------------------------- CUDA-core kernel --
+// One CTA: a query tile of SR = 16 pairs of one (sequence, cache head) and one
+// chunk of its keys; each of 4 warps owns 4 pairs. K and V tiles of STK = 32
+// keys are staged in shared memory as fp32 (dequantised there). Scores: lane =
+// key, so a K row is read once as float4s (row stride D + 4: conflict-free)
+// for 4 pairs whose q values are broadcast reads, 16 FMAs per 5 shared loads.
+// P V: lane = dim, each V element serving the warp's 4 pairs. All arithmetic is
+// fp32, as the fp32 model's parity with the reference needs (tensor-core TF32
+// does not reach it).
+constexpr int SR = 16;
+constexpr int STK = 32;
+constexpr int S_WARPS = 4;
+constexpr int S_ROWS = SR / S_WARPS;
+
+template <typename KV>
+__device__ __forceinline__ void load4(const KV* p, bool vec, int left, float (&f)[4]) {
+  if constexpr (std::is_same<KV, uint8_t>::value) {
+    if (vec) {
+      e4m3x4_to_float(*reinterpret_cast<const uint32_t*>(p), f);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = i < left ? f16x2_to_float2(cvt_e4m3x2_f16x2(p[i])).x : 0.f;
+  } else {
+    if (vec) {
+      if constexpr (sizeof(KV) == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        const KV* h = reinterpret_cast<const KV*>(&x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = to_f(h[i]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = i < left ? to_f(p[i]) : 0.f;
+  }
+}
+
+// DC: 32-dim columns per lane (head dim up to 32 DC).
+template <typename T, typename KV, int DC>
+__global__ void __launch_bounds__(S_WARPS * 32)
+paged_simt_kernel(const Params p, const bool vec) {
+  constexpr bool FP8 = std::is_same<KV, uint8_t>::value;
+  extern __shared__ float sm[];
+  const int D = p.D, Dp = (D + 3) & ~3, ldk = Dp + 4;
+  float* sQ = sm;                    // [SR][Dp]
+  float* sK = sQ + SR * Dp;          // [STK][ldk]
+  float* sV = sK + STK * ldk;        // [STK][Dp]
+  float* sP = sV + STK * Dp;         // [SR][STK]
+  int* sOk = reinterpret_cast<int*>(sP + SR * STK);  // [STK]: the key was loaded
+
+  const int s = blockIdx.z;
+  const Seq q = load_seq(p, s);
+  // blockIdx.x runs over (cache head, chunk), blockIdx.y over query tiles.
+  const int hk = blockIdx.x / p.P, chunk = blockIdx.x % p.P;
+  const int pairs = q.n * p.G, tile = blockIdx.y;
+  if (tile * SR >= pairs) return;
+  int pos_lo, pos_hi;
+  tile_positions(p, q, tile, SR, pos_lo, pos_hi);
+  const KeySpan span(p, q, pos_lo, pos_hi, STK);
+  const int per = p.chunk / STK, tiles = span.count();
+  const int chunks = chunks_of(p, tiles, STK);
+  if (chunk >= chunks) return;
+  const int v0 = chunk * per, v1 = chunk + 1 == chunks ? tiles : min(tiles, v0 + per);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < SR * Dp; i += blockDim.x) {
+    const int r = tile * SR + i / Dp, d = i % Dp;
+    float x = 0.f;
+    if (r < pairs && d < D)
+      x = to_f(static_cast<const T*>(p.q)[(int64_t)(q.row0 + r / p.G) * p.sq_t +
+                                          (int64_t)(hk * p.G + r % p.G) * p.sq_h + d]);
+    sQ[i] = x;
+  }
+  int pos[S_ROWS];
+#pragma unroll
+  for (int r = 0; r < S_ROWS; ++r) {
+    const int pr = tile * SR + warp * S_ROWS + r;
+    pos[r] = pr < pairs ? q.pos0 + pr / p.G : -1;  // position -1 sees nothing
+  }
+  float m[S_ROWS], l[S_ROWS], acc[S_ROWS][DC];
+#pragma unroll
+  for (int r = 0; r < S_ROWS; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) acc[r][c] = 0.f;
+  }
+  const int32_t* bt = p.block_tables + (int64_t)s * p.max_blocks;
+  const int bs = 1 << p.bs_log2;
+
+  for (int v = v0; v < v1; ++v) {
+    const int key0 = span.tile(v) * STK;
+    __syncthreads();  // the previous tile (and, at first, nothing) has been read
+    const int d4 = Dp / 4;
+    for (int i = threadIdx.x; i < STK * d4; i += blockDim.x) {
+      const int j = i / d4, d = (i % d4) * 4, key = key0 + j;
+      const int blk =
+          seen_by_any(p, pos_lo, pos_hi, q.ctx, key) ? bt[key >> p.bs_log2] : -1;
+      const bool ok = blk >= 0 && blk < p.num_blocks;
+      float fk[4] = {0.f, 0.f, 0.f, 0.f}, fv[4] = {0.f, 0.f, 0.f, 0.f};
+      if (ok) {
+        const int64_t cell = ((int64_t)blk * p.Hkv + hk) * bs + (key & (bs - 1));
+        load4(static_cast<const KV*>(p.k_cache) + cell * D + d, vec, D - d, fk);
+        load4(static_cast<const KV*>(p.v_cache) + cell * D + d, vec, D - d, fv);
+        if constexpr (FP8) {
+          const float ks = e8m0_to_float(p.k_scale[cell]), vs = e8m0_to_float(p.v_scale[cell]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { fk[e] *= ks; fv[e] *= vs; }
+        }
+      }
+      *reinterpret_cast<float4*>(sK + j * ldk + d) = make_float4(fk[0], fk[1], fk[2], fk[3]);
+      *reinterpret_cast<float4*>(sV + j * Dp + d) = make_float4(fv[0], fv[1], fv[2], fv[3]);
+      if (d == 0) sOk[j] = ok;
+    }
+    __syncthreads();
+    float sc[S_ROWS] = {};
+    for (int d = 0; d < Dp; d += 4) {
+      const float4 kx = *reinterpret_cast<const float4*>(sK + lane * ldk + d);
+#pragma unroll
+      for (int r = 0; r < S_ROWS; ++r) {
+        const float4 qx = *reinterpret_cast<const float4*>(sQ + (warp * S_ROWS + r) * Dp + d);
+        sc[r] = fmaf(qx.x, kx.x, sc[r]);
+        sc[r] = fmaf(qx.y, kx.y, sc[r]);
+        sc[r] = fmaf(qx.z, kx.z, sc[r]);
+        sc[r] = fmaf(qx.w, kx.w, sc[r]);
+      }
+    }
+    const bool key_ok = sOk[lane] != 0;
+#pragma unroll
+    for (int r = 0; r < S_ROWS; ++r) {
+      const float x = key_ok && sees(p, pos[r], q.ctx, key0 + lane) ? sc[r] * p.scale_log2 : -INFINITY;
+      // A NaN score stays visible: fmaxf drops it, but exp2f below returns it.
+      const float mx = fmaxf(m[r], warp_max(x));
+      const float m_use = mx == -INFINITY ? 0.f : mx;
+      const float a = exp2f(m[r] - m_use);
+      const float e = exp2f(x - m_use);
+      m[r] = mx;
+      l[r] = l[r] * a + e;  // per-lane partial sum
+#pragma unroll
+      for (int c = 0; c < DC; ++c) acc[r][c] *= a;
+      sP[(warp * S_ROWS + r) * STK + lane] = e;
+    }
+    __syncwarp();
+    for (int j = 0; j < STK; j += 4) {
+      float4 pr[S_ROWS];
+#pragma unroll
+      for (int r = 0; r < S_ROWS; ++r)
+        pr[r] = *reinterpret_cast<const float4*>(sP + (warp * S_ROWS + r) * STK + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const int d = c * 32 + lane;
+          const float vx = d < Dp ? sV[(j + e) * Dp + d] : 0.f;
+#pragma unroll
+          for (int r = 0; r < S_ROWS; ++r) {
+            const float pe = e == 0 ? pr[r].x : e == 1 ? pr[r].y : e == 2 ? pr[r].z : pr[r].w;
+            acc[r][c] = fmaf(pe, vx, acc[r][c]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < S_ROWS; ++r) {
+    const int pr = tile * SR + warp * S_ROWS + r;
+    if (pr >= pairs) continue;
+    const int row = q.row0 + pr / p.G, h = hk * p.G + pr % p.G;
+    const float lsum = warp_sum(l[r]);
+    const float inv = lsum > 0.f || lsum != lsum ? 1.f / lsum : 0.f;  // NaN sums give NaN
+    const float lse2 = lsum == 0.f ? -INFINITY : m[r] + log2f(lsum);
+    if (chunks == 1) {
+      T* dst = static_cast<T*>(p.o) + (int64_t)row * p.so_t + (int64_t)h * p.so_h;
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+        if (c * 32 + lane < D) dst[c * 32 + lane] = from_f<T>(acc[r][c] * inv);
+      if (p.lse != nullptr && lane == 0) p.lse[(int64_t)h * p.T + row] = lse2 * 0.69314718055994531f;
+    } else {
+      const int64_t at = ((int64_t)row * p.Hq + h) * p.P + chunk;
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+        if (c * 32 + lane < D) p.part_o[at * D + c * 32 + lane] = acc[r][c] * inv;
+      if (lane == 0) p.part_lse[at] = lse2;
+    }
+  }
+}
+
+int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
+  const int Dp = (p.D + 3) & ~3;
+  const size_t smem = sizeof(float) * (SR * Dp + STK * (Dp + 4) + STK * Dp + SR * STK + STK);
+  const int64_t tiles = ((int64_t)p.max_q * p.G + SR - 1) / SR;
+  LSB_CHECK_ARG(tiles <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff,
+                "paged_attn: %lld query tiles per head exceed 65535 (CUDA-core kernel)", (long long)tiles);
+  const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)tiles, (unsigned)p.S);
+  auto go = [&](auto tag, auto kvtag, auto dc) -> int {
+    using T = decltype(tag);
+    using KV = decltype(kvtag);
+    constexpr int DC = decltype(dc)::value;
+    // 4-element loads: every cache row starts on such a boundary.
+    const bool vec = p.D % 4 == 0 &&
+                     ((reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) &
+                      (4 * sizeof(KV) - 1)) == 0;
+    auto kern = paged_simt_kernel<T, KV, DC>;
+    static SmemLimit limit;
+    if (smem > 48 * 1024)
+      if (int rc = limit.ensure(kern, smem, "paged_attn smem attribute")) return rc;
+    kern<<<grid, S_WARPS * 32, smem, st>>>(p, vec);
+    LSB_CHECK_LAUNCH("paged_attn");
+    return LSB_OK;
+  };
+  auto by_dim = [&](auto tag, auto kvtag) -> int {
+    if (p.D <= 64) return go(tag, kvtag, std::integral_constant<int, 2>{});
+    if (p.D <= 128) return go(tag, kvtag, std::integral_constant<int, 4>{});
+    return go(tag, kvtag, std::integral_constant<int, 8>{});
+  };
+  return LSB_DISPATCH_DTYPE(dtype, T, [&] {
+    if (kv_fp8) return by_dim(T{}, uint8_t{});
+    return by_dim(T{}, T{});
+  });
+}
+
+// ----------------------------------------------------------------- combine --
+// One warp per (row, head): the grid is (row, head) pairs of the longest
+// sequence by sequences, so no row has to look its sequence up.
+constexpr int C_WARPS = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(C_WARPS * 32)
+paged_combine_kernel(const Params p, int R, int tk) {
+  allow_dependents();
+  wait_prerequisites();
+  const Seq q = load_seq(p, blockIdx.y);
+  const int id = blockIdx.x * C_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int i = id / p.Hq, h = id % p.Hq;
+  if (i >= q.n) return;
+  int pos_lo, pos_hi;
+  tile_positions(p, q, (i * p.G + h % p.G) / R, R, pos_lo, pos_hi);
+  const KeySpan span(p, q, pos_lo, pos_hi, tk);
+  const int chunks = chunks_of(p, span.count(), tk);
+  if (chunks == 1) return;
+  const int row = q.row0 + i;
+  const int64_t at = ((int64_t)row * p.Hq + h) * p.P;
+  float mx = -INFINITY;
+  bool nan = false;
+  for (int c = lane; c < chunks; c += 32) {
+    const float x = p.part_lse[at + c];
+    nan |= x != x;
+    mx = fmaxf(mx, x);
+  }
+  mx = warp_max(mx);
+  nan = __any_sync(0xffffffffu, nan);
+  const float m_use = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  for (int c = lane; c < chunks; c += 32) sum += exp2f(p.part_lse[at + c] - m_use);
+  sum = warp_sum(sum);
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  T* dst = static_cast<T*>(p.o) + (int64_t)row * p.so_t + (int64_t)h * p.so_h;
+  for (int d = lane; d < p.D; d += 32) {
+    float a = 0.f;
+    for (int c = 0; c < chunks; ++c)
+      a = fmaf(exp2f(p.part_lse[at + c] - m_use), p.part_o[(at + c) * p.D + d], a);
+    dst[d] = from_f<T>(nan ? __int_as_float(0x7fc00000) : a * inv);
+  }
+  if (p.lse != nullptr && lane == 0)
+    p.lse[(int64_t)h * p.T + row] =
+        nan ? __int_as_float(0x7fc00000)
+            : (sum > 0.f ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY);
+}
+
+int launch_combine(const Params& p, int rows_per_tile, int tk, int dtype, cudaStream_t st) {
+  const int64_t blocks = ((int64_t)p.max_q * p.Hq + C_WARPS - 1) / C_WARPS;
+  LSB_CHECK_ARG(blocks <= 0x7fffffff, "paged_attn: too many rows to combine");
+  return LSB_DISPATCH_DTYPE(dtype, T, [&] {
+    LSB_CUDA_OK(launch_kernel(paged_combine_kernel<T>, dim3((unsigned)blocks, (unsigned)p.S),
+                              dim3(C_WARPS * 32), 0, st, p, rows_per_tile, tk),
+                "paged_attn combine");
+    return LSB_OK;
+  });
+}
+
+// -------------------------------------------------------------- dispatch ---
+// How a call's keys are cut, from its sizes alone: with fewer query tiles
+// than the GPU holds CTAs (4 of them on each of a B200's 148 SMs for the
+// CUDA-core kernel), each tile's keys go to P CTAs of `chunk` keys.
+struct Plan {
+  int chunk, P;
+};
+
+static Plan plan_split(int64_t tiles, int64_t max_keys, int64_t want, int64_t min_chunk) {
+  int64_t P = tiles > 0 ? std::max<int64_t>(1, want / tiles) : 1;
+  int64_t chunk = (max_keys + P - 1) / P;
+  chunk = std::max<int64_t>(min_chunk, (chunk + 127) / 128 * 128);
+  P = std::max<int64_t>(1, (max_keys + chunk - 1) / chunk);
+  return {(int)std::min<int64_t>(chunk, 1 << 30), (int)P};
+}
+
+// Keys a row tile may visit: the block table's capacity, or with a window the
+// window, the tile's own rows and the sinks (each rounded up to a key tile).
+static int64_t max_visible(int64_t max_q, int64_t max_keys, int64_t window, int64_t sinks) {
+  if (window <= 0) return max_keys;
+  return std::min<int64_t>(max_keys, window + max_q + sinks + 3 * 128);
+}
+
+static Plan plan_simt(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t keys) {
+  return plan_split(S * Hkv * ((max_q * G + SR - 1) / SR), keys, 4 * 148, 128);
+}
+
+}  // namespace pa
+}  // namespace lsb
+
+extern "C" int64_t lsb_paged_attn_workspace_size(int64_t num_seqs, int64_t total_q,
+                                                 int64_t max_seqlen_q, int64_t Hq, int64_t Hkv,
+                                                 int64_t D, int64_t max_blocks_per_seq,
+                                                 int64_t block_size, int64_t window,
+                                                 int64_t num_sinks) {
+  using namespace lsb::pa;
+  if (num_seqs <= 0 || total_q <= 0 || max_seqlen_q <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 ||
+      D <= 0 || max_blocks_per_seq <= 0 || block_size <= 0)
+    return 0;
+  const int64_t keys =
+      max_visible(max_seqlen_q, max_blocks_per_seq * block_size, window, num_sinks);
+  const int64_t P = plan_simt(num_seqs, max_seqlen_q, Hkv, Hq / Hkv, keys).P;
+  if (P <= 1) return 0;
+  return lsb::align256(4 * total_q * Hq * P) + 4 * total_q * Hq * P * D;
+}
+
+extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_cache,
+                              const void* k_scale, const void* v_scale,
+                              const int32_t* block_tables, const int32_t* context_lens,
+                              const int32_t* cu_seqlens_q, void* o, float* lse, int64_t num_seqs,
+                              int64_t total_q, int64_t max_seqlen_q, int64_t Hq, int64_t Hkv,
+                              int64_t D, int64_t max_blocks_per_seq, int64_t block_size,
+                              int64_t num_blocks, int64_t sq_t, int64_t sq_h, int64_t so_t,
+                              int64_t so_h, int64_t window, int64_t num_sinks, float scale,
+                              int dtype, int kv_dtype, int impl, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  using namespace lsb::pa;
+  LSB_CHECK_ARG(num_seqs >= 0 && total_q >= 0 && max_seqlen_q >= 0 && Hq > 0 && Hkv > 0 && D > 0 &&
+                    max_blocks_per_seq > 0 && num_blocks > 0,
+                "paged_attn: bad sizes num_seqs=%lld total_q=%lld max_seqlen_q=%lld Hq=%lld Hkv=%lld "
+                "D=%lld max_blocks=%lld num_blocks=%lld",
+                (long long)num_seqs, (long long)total_q, (long long)max_seqlen_q, (long long)Hq,
+                (long long)Hkv, (long long)D, (long long)max_blocks_per_seq, (long long)num_blocks);
+  LSB_CHECK_ARG(Hq % Hkv == 0, "paged_attn: %lld query heads are no multiple of the cache's %lld",
+                (long long)Hq, (long long)Hkv);
+  LSB_CHECK_ARG(block_size > 0 && (block_size & (block_size - 1)) == 0,
+                "paged_attn: block_size %lld must be a power of two", (long long)block_size);
+  const int esz = lsb::dtype_size(dtype);
+  LSB_CHECK_ARG(esz > 0, "paged_attn: unsupported dtype %d", dtype);
+  const bool fp8 = kv_dtype == LSB_DTYPE_E4M3;
+  LSB_CHECK_ARG(fp8 || kv_dtype == dtype, "paged_attn: the cache holds q's type or e4m3, got %d", kv_dtype);
+  LSB_CHECK_ARG(window >= 0 && num_sinks >= 0 && (window > 0 || num_sinks == 0),
+                "paged_attn: window %lld and num_sinks %lld: neither is negative, and sinks need a window",
+                (long long)window, (long long)num_sinks);
+  LSB_CHECK_ARG(max_seqlen_q <= total_q, "paged_attn: max_seqlen_q %lld above total_q %lld",
+                (long long)max_seqlen_q, (long long)total_q);
+  LSB_CHECK_ARG(cu_seqlens_q != nullptr || total_q == num_seqs,
+                "paged_attn: without cu_seqlens_q there is one row per sequence");
+  if (num_seqs == 0 || total_q == 0 || max_seqlen_q == 0) return LSB_OK;
+  LSB_CHECK_ARG(q && k_cache && v_cache && block_tables && context_lens && o,
+                "paged_attn: null pointer");
+  LSB_CHECK_ARG(!fp8 || (k_scale && v_scale), "paged_attn: an e4m3 cache needs its scales");
+  constexpr int64_t kMax = 1LL << 30;
+  LSB_CHECK_ARG(num_seqs <= 65535 && total_q < kMax && Hq < 65536 && num_blocks < kMax &&
+                    total_q * Hq < kMax && max_blocks_per_seq < kMax && block_size < kMax &&
+                    max_blocks_per_seq * block_size < kMax,
+                "paged_attn: sizes too large (65535 sequences; 2^30 rows x heads, blocks, keys per "
+                "sequence)");
+  if (D > 256) {
+    lsb::set_error("paged_attn: head dim %lld above 256", (long long)D);
+    return LSB_ERR_UNSUPPORTED;
+  }
+  LSB_CHECK_ARG(impl == LSB_IMPL_AUTO || impl == LSB_IMPL_SIMT, "paged_attn: bad impl %d", impl);
+
+  Params p = {};
+  p.q = q; p.k_cache = k_cache; p.v_cache = v_cache;
+  p.k_scale = static_cast<const uint8_t*>(k_scale);
+  p.v_scale = static_cast<const uint8_t*>(v_scale);
+  p.block_tables = block_tables; p.context_lens = context_lens; p.cu_seqlens_q = cu_seqlens_q;
+  p.o = o; p.lse = lse;
+  p.sq_t = sq_t; p.sq_h = sq_h; p.so_t = so_t; p.so_h = so_h;
+  p.S = (int)num_seqs; p.T = (int)total_q; p.max_q = (int)max_seqlen_q;
+  p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv); p.D = (int)D;
+  p.max_blocks = (int)max_blocks_per_seq; p.num_blocks = (int)num_blocks;
+  while ((1LL << p.bs_log2) < block_size) ++p.bs_log2;
+  // A window or sinks past every position change nothing.
+  p.window = (int)std::min<int64_t>(window, kMax);
+  p.sinks = (int)std::min<int64_t>(num_sinks, kMax);
+  p.scale_log2 = scale * LOG2E;
+  const int64_t keys = max_visible(max_seqlen_q, max_blocks_per_seq * block_size, p.window, p.sinks);
+  const Plan plan = plan_simt(num_seqs, max_seqlen_q, Hkv, p.G, keys);
+  p.chunk = plan.chunk;
+  p.P = plan.P;
+  if (p.P > 1) {
+    const int64_t need = lsb_paged_attn_workspace_size(num_seqs, total_q, max_seqlen_q, Hq, Hkv, D,
+                                                       max_blocks_per_seq, block_size, window,
+                                                       num_sinks);
+    LSB_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && lsb::aligned16(workspace),
+                  "paged_attn: workspace of %lld bytes (16-byte aligned) required, got %lld",
+                  (long long)need, (long long)workspace_bytes);
+    p.part_lse = static_cast<float*>(workspace);
+    p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                        lsb::align256(4 * total_q * Hq * p.P));
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  int rc = launch_simt(p, dtype, fp8, st);
+  if (rc == LSB_OK && p.P > 1) rc = launch_combine(p, SR, STK, dtype, st);
+  return rc;
+}

@@ -18,6 +18,7 @@ import math
 import torch
 
 from .. import _lib
+from .paged_chunk_attention import _paged_attn, paged_chunk_workspace
 
 
 def write_kv_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -44,9 +45,16 @@ def write_kv_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_ca
     _lib.check(rc, "lsb_kv_cache_write")
 
 
-def paged_decode_workspace(q_shape, max_blocks_per_seq: int, block_size: int, device) -> torch.Tensor:
-    """fp32 scratch for split-context partials (empty when none is needed)."""
+def paged_decode_workspace(q_shape, max_blocks_per_seq: int, block_size: int, device, *,
+                           num_kv_heads: int | None = None, quantized: bool = False,
+                           window: int | None = None, num_sinks: int = 0) -> torch.Tensor:
+    """fp32 scratch for split-context partials (empty when none is needed). The
+    keyword arguments say how ``paged_decode_attention`` will be called:
+    the cache's heads where they are fewer than q's, an e4m3 cache, a window."""
     S, H, D = q_shape
+    if quantized or window is not None or num_kv_heads not in (None, H):
+        return paged_chunk_workspace(q_shape, S, 1, num_kv_heads or H, max_blocks_per_seq, block_size,
+                                     device, window, num_sinks)
     nbytes = _lib.load().lsb_paged_decode_workspace_size(S, H, D, max_blocks_per_seq, block_size)
     return torch.empty(max(nbytes // 4, 1), dtype=torch.float32, device=device)
 
@@ -54,7 +62,9 @@ def paged_decode_workspace(q_shape, max_blocks_per_seq: int, block_size: int, de
 def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                            block_tables: torch.Tensor, context_lens: torch.Tensor,
                            scale: float | None = None, out: torch.Tensor | None = None,
-                           workspace: torch.Tensor | None = None) -> torch.Tensor:
+                           workspace: torch.Tensor | None = None, *, window: int | None = None,
+                           num_sinks: int = 0, k_scale: torch.Tensor | None = None,
+                           v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """o[s, h] = softmax(q[s, h] . K[s, h, :L_s]^T * scale) V[s, h, :L_s].
 
     q: [S, H, D]; k_cache, v_cache: [num_blocks, H, block_size, D];
@@ -62,9 +72,19 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     in the cache, including the current one). scale defaults to 1/sqrt(D).
     Passing ``out`` and ``workspace`` makes the call allocation-free (for CUDA
     graph capture).
+
+    ``window`` limits each sequence to its last ``window`` tokens (the current
+    one among them) and its first ``num_sinks``; ``k_scale``/``v_scale`` say that the
+    caches are quantised (``quantize_kv_cache``); q may have a multiple of the
+    caches' heads. Such a call is ``paged_chunk_attention`` of one token per
+    sequence (``paged_decode_workspace`` takes the same keywords).
     """
     assert q.ndim == 3, f"q must be [S, H, D], got {q.ndim}D"
     S, H, D = q.shape
+    if (window is not None or num_sinks or k_scale is not None or v_scale is not None
+            or (k_cache.ndim == 4 and k_cache.shape[1] != H)):
+        return _paged_attn(q, k_cache, v_cache, block_tables, context_lens, None, 1, window, num_sinks,
+                           k_scale, v_scale, scale, out, None, workspace)
     assert k_cache.ndim == 4 and k_cache.shape == v_cache.shape, "caches must be [num_blocks, H, block_size, D]"
     nb, Hc, bs, Dc = k_cache.shape
     assert (Hc, Dc) == (H, D), f"cache heads/dim {(Hc, Dc)} do not match q {(H, D)}"
