@@ -47,6 +47,9 @@ extern "C" {
 #define LSB_IMPL_SIMT 1    /* CUDA-core kernel, any dtype / head dim <= 256  */
 #define LSB_IMPL_TCGEN05 2 /* tcgen05 + TMEM + TMA kernel; error if ineligible */
 
+/* lsb_paged_attn only: the warp-level MMA kernel for a few rows per sequence. */
+#define LSB_IMPL_ROWS 3
+
 /* Message describing the last failure on this thread ("" if none). */
 LSB_API const char* lsb_last_error(void);
 

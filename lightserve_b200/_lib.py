@@ -31,6 +31,7 @@ DTYPE_E4M3 = 3  # quantised KV caches only
 IMPL_AUTO = 0
 IMPL_SIMT = 1
 IMPL_TCGEN05 = 2
+IMPL_ROWS = 3  # lsb_paged_attn only
 
 _DTYPE_CODES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
 

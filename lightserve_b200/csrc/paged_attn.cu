@@ -322,6 +322,19 @@ static Plan plan_simt(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t 
   return plan_split(S * Hkv * ((max_q * G + SR - 1) / SR), keys, 4 * 148, 128);
 }
 
+// Pairs up to which the few-rows kernel is taken where it serves the call.
+constexpr int64_t ROWS_MAX_PAIRS = 64;
+
+static Plan plan_rows(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t keys) {
+  if (max_q * G > ROWS_MAX_PAIRS) return {1 << 30, 1};
+  const int64_t tiles = S * Hkv * ((max_q * G + ROWS_R - 1) / ROWS_R);
+  const int64_t P = std::max<int64_t>(1, 12 * 148 / tiles);
+  int64_t chunk = std::min<int64_t>(512, ((keys + P - 1) / P + 127) / 128 * 128);
+  chunk = std::max<int64_t>(chunk, (keys / std::max<int64_t>(64, P) + 127) / 128 * 128);
+  return {(int)std::min<int64_t>(chunk, 1 << 30),
+          (int)std::max<int64_t>(1, (keys + chunk - 1) / chunk)};
+}
+
 }  // namespace pa
 }  // namespace lsb
 
@@ -336,7 +349,9 @@ extern "C" int64_t lsb_paged_attn_workspace_size(int64_t num_seqs, int64_t total
     return 0;
   const int64_t keys =
       max_visible(max_seqlen_q, max_blocks_per_seq * block_size, window, num_sinks);
-  const int64_t P = plan_simt(num_seqs, max_seqlen_q, Hkv, Hq / Hkv, keys).P;
+  const int64_t G = Hq / Hkv;
+  const int64_t P = std::max(plan_simt(num_seqs, max_seqlen_q, Hkv, G, keys).P,
+                             plan_rows(num_seqs, max_seqlen_q, Hkv, G, keys).P);
   if (P <= 1) return 0;
   return lsb::align256(4 * total_q * Hq * P) + 4 * total_q * Hq * P * D;
 }
@@ -387,7 +402,8 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
     lsb::set_error("paged_attn: head dim %lld above 256", (long long)D);
     return LSB_ERR_UNSUPPORTED;
   }
-  LSB_CHECK_ARG(impl == LSB_IMPL_AUTO || impl == LSB_IMPL_SIMT, "paged_attn: bad impl %d", impl);
+  LSB_CHECK_ARG(impl == LSB_IMPL_AUTO || impl == LSB_IMPL_SIMT || impl == LSB_IMPL_ROWS,
+                "paged_attn: bad impl %d", impl);
 
   Params p = {};
   p.q = q; p.k_cache = k_cache; p.v_cache = v_cache;
@@ -405,7 +421,15 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
   p.sinks = (int)std::min<int64_t>(num_sinks, kMax);
   p.scale_log2 = scale * LOG2E;
   const int64_t keys = max_visible(max_seqlen_q, max_blocks_per_seq * block_size, p.window, p.sinks);
-  const Plan plan = plan_simt(num_seqs, max_seqlen_q, Hkv, p.G, keys);
+  Plan plan = plan_rows(num_seqs, max_seqlen_q, Hkv, p.G, keys);
+  p.P = plan.P;
+  const bool rows_ok = rows_eligible(p, dtype, fp8);
+  LSB_CHECK_ARG(impl != LSB_IMPL_ROWS || rows_ok,
+                "paged_attn: the few-rows kernel needs bf16/fp16, D in {64,128}, pages of 8 keys or "
+                "more, q strides that are multiples of 4 elements and 16-byte aligned caches");
+  const bool rows = impl == LSB_IMPL_ROWS ||
+                    (impl == LSB_IMPL_AUTO && rows_ok && max_seqlen_q * p.G <= ROWS_MAX_PAIRS);
+  if (!rows) plan = plan_simt(num_seqs, max_seqlen_q, Hkv, p.G, keys);
   p.chunk = plan.chunk;
   p.P = plan.P;
   if (p.P > 1) {
@@ -420,7 +444,7 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
                                         lsb::align256(4 * total_q * Hq * p.P));
   }
   cudaStream_t st = (cudaStream_t)stream;
-  int rc = launch_simt(p, dtype, fp8, st);
-  if (rc == LSB_OK && p.P > 1) rc = launch_combine(p, SR, STK, dtype, st);
-  return rc;
+  const int rc = rows ? launch_rows(p, dtype, fp8, st) : launch_simt(p, dtype, fp8, st);
+  if (rc != LSB_OK || p.P == 1) return rc;
+  return rows ? launch_combine(p, ROWS_R, ROWS_TK, dtype, st) : launch_combine(p, SR, STK, dtype, st);
 }

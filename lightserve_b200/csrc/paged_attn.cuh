@@ -129,5 +129,9 @@ int launch_combine(const Params& p, int rows_per_tile, int tk, int dtype, cudaSt
 // Each kernel's launcher. `kv_fp8`: the cache holds e4m3.
 int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 
+constexpr int ROWS_R = 16, ROWS_TK = 16;  // paged_attn_rows.cu's query tile and key group
+bool rows_eligible(const Params& p, int dtype, bool kv_fp8);
+int launch_rows(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
+
 }  // namespace pa
 }  // namespace lsb

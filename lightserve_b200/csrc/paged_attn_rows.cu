@@ -1,0 +1,524 @@
+// Paged attention for a few rows per sequence (decode, drafted tokens): the
+// cache is read once at HBM speed, the arithmetic rides along on mma.sync.
+//
+// One CTA: a query tile of R = 16 pairs (row, head of the group) of one
+// (sequence, cache head) and one chunk of its keys; its 4 warps take groups of
+// 16 keys in turn and merge at the end. Bound by HBM: per 16 keys a warp moves
+// 4 KiB (e4m3, D = 128) and issues 32 m16n8k16 MMAs, whose row padding (15 of
+// 16 rows are empty for one query head) costs nothing that is scarce. The
+// warp-level MMA is the right size here: tcgen05's 128-row tiles would stage
+// every key through shared memory for one row of use.
+//
+// K and V go from global memory straight into MMA fragments, the next group's
+// loads in flight while the current one is computed; no shared memory, no
+// barriers in the loop. What makes that possible is that the contraction's
+// index order is free as long as both operands agree on it:
+//  * S = Q K^T: lane (g, t) = (lane / 4, lane % 4) loads 16-byte runs of key g's
+//    row at dims (4 i + t) EK and uses their 4-element pieces as its slots of
+//    consecutive k steps; Q is laid out by the same rule, once.
+//  * O += P V: the score fragment's columns (keys 2t, 2t + 1 of each half
+//    group) are P's A-operand slots as they stand. Lane (g, t) loads those four
+//    keys' V at dims (8 i + g) EV and interleaves pairs of keys with byte
+//    permutes into B fragments; output column g of n-tile j is dim
+//    (8 i + g) EV + e, j = i EV + e.
+//
+// e4m3 cache: bytes convert to fp16 in one instruction per pair (exactly; the
+// MMAs run in fp16), unscaled. K's power-of-two scale multiplies the score. V's
+// is added to the score as an exponent: w_j = 2^(x_j + e_j - m'), with a running
+// maximum m' of x + e of its own, so weights stay near 1 whatever the scales,
+// beside p_j = 2^(x_j - m) for the denominator. A bf16 q is scaled by a power
+// of two per row into fp16's range (exact down to 2^-28 of the row's largest
+// value; below that the error is under 2^-39 of it).
+//
+// The running maximum is raised only when a score exceeds it by 2^8 (a vote
+// per group instead of shuffles and a rescale). Weights carry a factor 2^7, so
+// an fp16 weight keeps its precision down to 2^-21 of the maximum and vanishes
+// below 2^-32: rounding P to 16 bits is off by half a step of the operand type
+// relative to each weight, as in the framework's other attention kernels.
+#include "paged_attn.cuh"
+#include "sm100.cuh"
+
+#include <type_traits>
+
+namespace lsb {
+namespace pa {
+
+namespace rows {
+
+constexpr int TK = 16;      // keys per group
+constexpr int WARPS = 4;
+constexpr float RAISE = 8.f;   // log2: how far a score may exceed the reference maximum
+constexpr float LIFT = 7.f;    // log2: factor on every weight
+
+template <bool F16>
+__device__ __forceinline__ void mma16816(float& c0, float& c1, float& c2, float& c3, uint32_t a0,
+                                         uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// N words from global memory, read once (16 bytes a load where N allows).
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const void* p) {
+  static_assert(N == 2 || N == 4, "8 or 16 bytes");
+  if constexpr (N == 4) {
+    const uint4 x = __ldcs(static_cast<const uint4*>(p));
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else {
+    const uint2 x = __ldcs(static_cast<const uint2*>(p));
+    w[0] = x.x; w[1] = x.y;
+  }
+}
+
+template <bool FP8, int D>
+struct Shape {
+  static constexpr int EB = FP8 ? 1 : 2;           // bytes per cached element
+  static constexpr int EK = 16 / EB;               // K elements per lane and load
+  static constexpr int NK = D / (4 * EK);          // K loads per key and lane
+  static constexpr int EV = FP8 ? D / 8 : 8;       // V elements per lane and load
+  static constexpr int NV = D / (8 * EV);          // V loads per key and lane
+  static constexpr int WV = EV * EB / 4;           // words per V load
+  static constexpr int STEPS = D / 16;             // k steps of S
+  static constexpr int NT = D / 8;                 // n-tiles of O
+};
+
+// One group's operands as they arrive: K rows of keys g and 8 + g, V rows of
+// keys 2t, 2t + 1, 8 + 2t, 8 + 2t + 1, and the scales of those four keys.
+template <bool FP8, int D>
+struct Group {
+  using S = Shape<FP8, D>;
+  uint32_t k[2][S::NK][4];
+  uint32_t v[4][S::NV][S::WV];
+  uint16_t ks[2], vs[2];
+  int tok0;
+  int ids[2];  // page of each half, -1: no such page
+};
+
+template <typename T, bool FP8, int D, bool R8>
+struct Occupancy {
+  // Resident CTAs the registers are budgeted for: two groups in flight take
+  // 64 (e4m3) or 128 registers, Q and O 48 (8 rows) or 96, at D = 128.
+  static constexpr int CTAS = D == 64 ? (FP8 && R8 ? 5 : 4) : (FP8 && R8 ? 3 : 2);
+};
+
+template <typename T, bool FP8, int D, bool R8>
+__global__ void __launch_bounds__(WARPS * 32, (Occupancy<T, FP8, D, R8>::CTAS))
+paged_rows_kernel(const Params p) {
+  allow_dependents();
+  wait_prerequisites();
+  using S = Shape<FP8, D>;
+  constexpr bool F16 = FP8 || std::is_same<T, __half>::value;  // MMA operand type
+  constexpr int ROWS = R8 ? 8 : 16;
+  constexpr int HALVES = R8 ? 1 : 2;
+  __shared__ float sm_acc[WARPS][ROWS][D];
+  __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS], sm_w[WARPS][ROWS];
+
+  const int chunk = blockIdx.x % p.P, hk = blockIdx.x / p.P, tile = blockIdx.y, s = blockIdx.z;
+  const Seq q = load_seq(p, s);
+  const int pairs = q.n * p.G;
+  if (tile * 16 >= pairs) return;
+  int pos_lo, pos_hi;
+  tile_positions(p, q, tile, 16, pos_lo, pos_hi);
+  const KeySpan span(p, q, pos_lo, pos_hi, TK);
+  const int tiles = span.count(), per = p.chunk / TK;
+  const int chunks = chunks_of(p, tiles, TK);
+  if (chunk >= chunks) return;
+  const int v0 = chunk * per, v1 = chunk + 1 == chunks ? tiles : min(tiles, v0 + per);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int32_t* bt = p.block_tables + (int64_t)s * p.max_blocks;
+  const int bs = 1 << p.bs_log2;
+
+  // ---------------------------------------------------------------- Q ----
+  uint32_t qa[HALVES][S::STEPS][2];
+  float fac[HALVES];  // score factor of the row: scale log2(e), and the row's power of two
+  int pos[HALVES];
+#pragma unroll
+  for (int hf = 0; hf < HALVES; ++hf) {
+    const int pr = tile * 16 + hf * 8 + g;
+    const bool in = pr < pairs;
+    pos[hf] = in ? q.pos0 + pr / p.G : -1;
+    const T* row = static_cast<const T*>(p.q) + (int64_t)(q.row0 + (in ? pr / p.G : 0)) * p.sq_t +
+                   (int64_t)(hk * p.G + (in ? pr % p.G : 0)) * p.sq_h;
+    uint2 raw[S::STEPS];
+#pragma unroll
+    for (int st = 0; st < S::STEPS; ++st) {
+      const int i = st / (S::EK / 4), w = st % (S::EK / 4);
+      raw[st] = in ? *reinterpret_cast<const uint2*>(row + (4 * i + t) * S::EK + 4 * w)
+                   : make_uint2(0u, 0u);
+    }
+    fac[hf] = p.scale_log2;
+    if constexpr (FP8 && std::is_same<T, __nv_bfloat16>::value) {
+      float amax = 0.f;
+#pragma unroll
+      for (int st = 0; st < S::STEPS; ++st) {
+        const T* x = reinterpret_cast<const T*>(&raw[st]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) amax = fmaxf(amax, finite_abs(to_f(x[e])));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // The row's largest value goes to [2^14, 2^15); biased exponent x,
+      // held where 2^(x - 141) and its inverse are normal.
+      const int x = min(max((int)(__float_as_uint(amax) >> 23), 16), 254);
+      const float down = __uint_as_float((uint32_t)(268 - x) << 23 & 0x7f800000u);  // 2^(141 - x)
+      fac[hf] *= __uint_as_float((uint32_t)max(x - 14, 1) << 23);                  // 2^(x - 141)
+#pragma unroll
+      for (int st = 0; st < S::STEPS; ++st) {
+        const T* y = reinterpret_cast<const T*>(&raw[st]);
+        qa[hf][st][0] = sm100::pack_f16(to_f(y[0]) * down, to_f(y[1]) * down);
+        qa[hf][st][1] = sm100::pack_f16(to_f(y[2]) * down, to_f(y[3]) * down);
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < S::STEPS; ++st) {
+        qa[hf][st][0] = raw[st].x;
+        qa[hf][st][1] = raw[st].y;
+      }
+    }
+  }
+
+  // ------------------------------------------------------------- loads ----
+  // Page ids of this warp's next 16 groups, one half group per lane.
+  auto fetch_ids = [&](int v) -> int {
+    const int vv = v + (lane >> 1) * WARPS;
+    if (vv >= v1) return -1;
+    const int tok = span.tile(vv) * TK + 8 * (lane & 1);
+    if (tok >= q.ctx) return -1;
+    const int id = bt[tok >> p.bs_log2];
+    return id >= 0 && id < p.num_blocks ? id : -1;
+  };
+  const uint8_t* kc = static_cast<const uint8_t*>(p.k_cache);
+  const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
+  auto load = [&](Group<FP8, D>& x, int v, int id0, int id1) {
+    x.tok0 = span.tile(v) * TK;
+    x.ids[0] = id0;
+    x.ids[1] = id1;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int id = x.ids[hf];
+      if (id >= 0) {
+        const int64_t cell = ((int64_t)id * p.Hkv + hk) * bs + ((x.tok0 + 8 * hf) & (bs - 1));
+        const uint8_t* kr = kc + (cell + g) * (D * S::EB) + t * 16;
+#pragma unroll
+        for (int i = 0; i < S::NK; ++i) load_words(x.k[hf][i], kr + i * 64);
+        const uint8_t* vr = vc + (cell + 2 * t) * (D * S::EB) + g * (S::EV * S::EB);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < S::NV; ++i)
+            load_words(x.v[2 * hf + e][i], vr + e * (D * S::EB) + i * (8 * S::EV * S::EB));
+        if constexpr (FP8) {
+          x.ks[hf] = *reinterpret_cast<const uint16_t*>(p.k_scale + cell + 2 * t);
+          x.vs[hf] = *reinterpret_cast<const uint16_t*>(p.v_scale + cell + 2 * t);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < S::NK; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) x.k[hf][i][w] = 0u;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+            for (int w = 0; w < S::WV; ++w) x.v[2 * hf + e][i][w] = 0u;
+        x.ks[hf] = x.vs[hf] = 0x7f7f;
+      }
+    }
+  };
+
+  // ----------------------------------------------------------- compute ----
+  float m[HALVES], mw[HALVES], l[HALVES], acc[S::NT][2 * HALVES];
+#pragma unroll
+  for (int hf = 0; hf < HALVES; ++hf) {
+    m[hf] = mw[hf] = -INFINITY;
+    l[hf] = 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 2 * HALVES; ++e) acc[j][e] = 0.f;
+
+  auto compute = [&](Group<FP8, D>& x) {
+    float sc[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+#pragma unroll
+    for (int st = 0; st < S::STEPS; ++st) {
+      const int i = st / (S::EK / 4), w = st % (S::EK / 4);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        uint32_t b0, b1;
+        if constexpr (FP8) {
+          b0 = cvt_e4m3x2_f16x2((uint16_t)(x.k[n][i][w] & 0xffff));
+          b1 = cvt_e4m3x2_f16x2((uint16_t)(x.k[n][i][w] >> 16));
+        } else {
+          b0 = x.k[n][i][2 * w];
+          b1 = x.k[n][i][2 * w + 1];
+        }
+        mma16816<F16>(sc[n][0], sc[n][1], sc[n][2], sc[n][3], qa[0][st][0],
+                      R8 ? 0u : qa[HALVES - 1][st][0], qa[0][st][1],
+                      R8 ? 0u : qa[HALVES - 1][st][1], b0, b1);
+      }
+    }
+    // Scores in log2 units; keys that a row does not see go to -inf.
+    const int last = x.tok0 + TK - 1;
+    const bool whole = last <= pos_lo && last < q.ctx && x.ids[0] >= 0 && x.ids[1] >= 0 &&
+                       (p.window == 0 || pos_hi - x.tok0 < p.window || last < p.sinks);
+    float ev[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float f = 1.f;
+        if constexpr (FP8) {
+          f = e8m0_to_float((x.ks[n] >> (8 * e)) & 0xff);
+          const int b = (x.vs[n] >> (8 * e)) & 0xff;
+          ev[n][e] = b == 255 ? __int_as_float(0x7fc00000) : (float)(b - 127);
+        }
+#pragma unroll
+        for (int hf = 0; hf < HALVES; ++hf) sc[n][2 * hf + e] *= fac[hf] * f;
+      }
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = x.tok0 + 8 * n + 2 * t + e;
+#pragma unroll
+          for (int hf = 0; hf < HALVES; ++hf)
+            if (x.ids[n] < 0 || !sees(p, pos[hf], q.ctx, j)) sc[n][2 * hf + e] = -INFINITY;
+          if (!seen_by_any(p, pos_lo, pos_hi, q.ctx, j)) {
+            ev[n][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+              for (int w = 0; w < S::WV; ++w) x.v[2 * n + e][i][w] = 0u;
+          }
+        }
+    }
+    bool raise = false;
+#pragma unroll
+    for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          raise |= sc[n][2 * hf + e] > m[hf] + RAISE;
+          if constexpr (FP8) raise |= sc[n][2 * hf + e] + ev[n][e] > mw[hf] + RAISE;
+        }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int hf = 0; hf < HALVES; ++hf) {
+        float a = m[hf], b = mw[hf];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            a = fmaxf(a, sc[n][2 * hf + e]);
+            if constexpr (FP8) b = fmaxf(b, sc[n][2 * hf + e] + ev[n][e]);
+          }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+          if constexpr (FP8) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+        }
+        if constexpr (!FP8) b = a;
+        const float ra = exp2f(m[hf] - (a == -INFINITY ? 0.f : a));
+        const float rb = exp2f(mw[hf] - (b == -INFINITY ? 0.f : b));
+        m[hf] = a;
+        mw[hf] = b;
+        l[hf] *= ra;
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+          acc[j][2 * hf] *= rb;
+          acc[j][2 * hf + 1] *= rb;
+        }
+      }
+    }
+    uint32_t pa[HALVES][2];  // P as A fragments: [row half][half group]
+#pragma unroll
+    for (int hf = 0; hf < HALVES; ++hf) {
+      const float mm = m[hf] == -INFINITY ? 0.f : m[hf] - LIFT;
+      const float mmw = mw[hf] == -INFINITY ? 0.f : mw[hf] - LIFT;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float p0 = sm100::ex2(sc[n][2 * hf] - mm), p1 = sm100::ex2(sc[n][2 * hf + 1] - mm);
+        l[hf] += p0 + p1;
+        if constexpr (FP8)
+          pa[hf][n] = sm100::pack_f16(sm100::ex2(sc[n][2 * hf] + (ev[n][0] - mmw)),
+                                      sm100::ex2(sc[n][2 * hf + 1] + (ev[n][1] - mmw)));
+        else
+          pa[hf][n] = F16 ? sm100::pack_f16(p0, p1) : sm100::pack_bf16(p0, p1);
+      }
+    }
+    auto pv = [&](int j, uint32_t b0, uint32_t b1) {
+      float z0 = 0.f, z1 = 0.f;  // rows 8-15 of an 8-row tile
+      mma16816<F16>(acc[j][0], acc[j][1], R8 ? z0 : acc[j][2 * HALVES - 2],
+                    R8 ? z1 : acc[j][2 * HALVES - 1], pa[0][0], R8 ? 0u : pa[HALVES - 1][0],
+                    pa[0][1], R8 ? 0u : pa[HALVES - 1][1], b0, b1);
+    };
+#pragma unroll
+    for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+      for (int w = 0; w < S::WV; ++w) {
+        const uint32_t a = x.v[0][i][w], b = x.v[1][i][w], c = x.v[2][i][w], d = x.v[3][i][w];
+        if constexpr (FP8) {
+          const int j = i * S::EV + 4 * w;
+          const uint32_t lo0 = __byte_perm(a, b, 0x5140), lo1 = __byte_perm(c, d, 0x5140);
+          const uint32_t hi0 = __byte_perm(a, b, 0x7362), hi1 = __byte_perm(c, d, 0x7362);
+          pv(j, cvt_e4m3x2_f16x2((uint16_t)(lo0 & 0xffff)), cvt_e4m3x2_f16x2((uint16_t)(lo1 & 0xffff)));
+          pv(j + 1, cvt_e4m3x2_f16x2((uint16_t)(lo0 >> 16)), cvt_e4m3x2_f16x2((uint16_t)(lo1 >> 16)));
+          pv(j + 2, cvt_e4m3x2_f16x2((uint16_t)(hi0 & 0xffff)), cvt_e4m3x2_f16x2((uint16_t)(hi1 & 0xffff)));
+          pv(j + 3, cvt_e4m3x2_f16x2((uint16_t)(hi0 >> 16)), cvt_e4m3x2_f16x2((uint16_t)(hi1 >> 16)));
+        } else {
+          const int j = i * S::EV + 2 * w;
+          pv(j, __byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
+          pv(j + 1, __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
+        }
+      }
+  };
+
+  {
+    int v = v0 + warp;
+    int ids = fetch_ids(v), at = 0;
+    auto next_ids = [&](int vv, int& a, int& b) {  // ids of group vv, the at-th of the fetched 16
+      if (at == 16) {
+        ids = fetch_ids(vv);
+        at = 0;
+      }
+      a = __shfl_sync(0xffffffffu, ids, 2 * at);
+      b = __shfl_sync(0xffffffffu, ids, 2 * at + 1);
+      ++at;
+    };
+    int a = -1, b = -1;
+    Group<FP8, D> cur, nxt;
+    if (v < v1) {
+      next_ids(v, a, b);
+      load(cur, v, a, b);
+    }
+    for (; v < v1; v += WARPS) {
+      const bool more = v + WARPS < v1;
+      if (more) {
+        next_ids(v + WARPS, a, b);
+        load(nxt, v + WARPS, a, b);
+      }
+      compute(cur);
+      if (more) cur = nxt;
+    }
+  }
+
+  // ------------------------------------------------------------- merge ----
+#pragma unroll
+  for (int hf = 0; hf < HALVES; ++hf) {
+    l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+    l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+    const int r = hf * 8 + g;
+    if (t == 0) {
+      sm_m[warp][r] = m[hf];
+      sm_l[warp][r] = l[hf];
+      sm_w[warp][r] = mw[hf];
+    }
+#pragma unroll
+    for (int i = 0; i < S::NV; ++i)
+#pragma unroll
+      for (int e = 0; e < S::EV; ++e) {
+        float* dst = &sm_acc[warp][r][(8 * i + 2 * t) * S::EV + e];
+        dst[0] = acc[i * S::EV + e][2 * hf];
+        dst[S::EV] = acc[i * S::EV + e][2 * hf + 1];
+      }
+  }
+  __syncthreads();
+  const int here = min(ROWS, pairs - tile * 16);
+  for (int r = warp; r < here; r += WARPS) {
+    float M = -INFINITY, MW = -INFINITY, L = 0.f, wt[WARPS];
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      M = fmaxf(M, sm_m[w][r]);
+      MW = fmaxf(MW, sm_w[w][r]);
+    }
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      L += sm_m[w][r] == -INFINITY ? sm_l[w][r] : exp2f(sm_m[w][r] - M) * sm_l[w][r];
+      wt[w] = sm_w[w][r] == -INFINITY ? 1.f : exp2f(sm_w[w][r] - MW);
+    }
+    // 2^(MW - M): V's scale, back on the result (1 for a 16-bit cache).
+    const float back = FP8 && MW != -INFINITY ? exp2f(MW - M) : 1.f;
+    const float inv = L > 0.f || L != L ? back / L : 0.f;  // NaN sums give NaN
+    const int pr = tile * 16 + r;
+    const int row = q.row0 + pr / p.G, h = hk * p.G + pr % p.G;
+    const float lse2 = L == 0.f ? -INFINITY : M + log2f(L) - LIFT;
+    const int64_t at = ((int64_t)row * p.Hq + h) * p.P + chunk;
+    T* dst = static_cast<T*>(p.o) + (int64_t)row * p.so_t + (int64_t)h * p.so_h;
+    for (int d = lane; d < D; d += 32) {
+      float a = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) a = fmaf(wt[w], sm_acc[w][r][d], a);
+      a *= inv;
+      if (chunks == 1)
+        dst[d] = from_f<T>(a);
+      else
+        p.part_o[at * D + d] = a;
+    }
+    if (lane == 0) {
+      if (chunks > 1)
+        p.part_lse[at] = lse2;
+      else if (p.lse != nullptr)
+        p.lse[(int64_t)h * p.T + row] = lse2 * 0.69314718055994531f;
+    }
+  }
+}
+
+template <typename T, bool FP8, int D>
+static int launch(const Params& p, cudaStream_t st) {
+  const int64_t pairs = (int64_t)p.max_q * p.G;
+  const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)((pairs + 15) / 16), (unsigned)p.S);
+  if (pairs <= 8)
+    LSB_CUDA_OK(launch_kernel(paged_rows_kernel<T, FP8, D, true>, grid, dim3(WARPS * 32), 0, st, p),
+                "paged_attn");
+  else
+    LSB_CUDA_OK(launch_kernel(paged_rows_kernel<T, FP8, D, false>, grid, dim3(WARPS * 32), 0, st, p),
+                "paged_attn");
+  return LSB_OK;
+}
+
+}  // namespace rows
+
+bool rows_eligible(const Params& p, int dtype, bool kv_fp8) {
+  if (dtype != LSB_DTYPE_BF16 && dtype != LSB_DTYPE_F16) return false;
+  if ((p.D != 64 && p.D != 128) || p.bs_log2 < 3) return false;
+  // q rows are read in 8-byte pieces, the cache in 8- and 16-byte ones, the
+  // scales in pairs.
+  auto at = [](const void* x, uintptr_t a) { return (reinterpret_cast<uintptr_t>(x) & (a - 1)) == 0; };
+  if (!at(p.q, 8) || p.sq_t % 4 != 0 || p.sq_h % 4 != 0) return false;
+  if (!at(p.k_cache, 16) || !at(p.v_cache, 16)) return false;
+  if (kv_fp8 && (!at(p.k_scale, 2) || !at(p.v_scale, 2))) return false;
+  return ((int64_t)p.max_q * p.G + 15) / 16 <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff;
+}
+
+int launch_rows(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
+  const bool bf = dtype == LSB_DTYPE_BF16;
+  if (p.D == 128) {
+    if (kv_fp8) return bf ? rows::launch<__nv_bfloat16, true, 128>(p, st) : rows::launch<__half, true, 128>(p, st);
+    return bf ? rows::launch<__nv_bfloat16, false, 128>(p, st) : rows::launch<__half, false, 128>(p, st);
+  }
+  if (kv_fp8) return bf ? rows::launch<__nv_bfloat16, true, 64>(p, st) : rows::launch<__half, true, 64>(p, st);
+  return bf ? rows::launch<__nv_bfloat16, false, 64>(p, st) : rows::launch<__half, false, 64>(p, st);
+}
+
+}  // namespace pa
+}  // namespace lsb

@@ -11,7 +11,8 @@ rounding to the output type, u32 = 2^-24.
 * Sums of N terms in fp32, the rescaling and the joining of split ranges:
   (N + 64) u32 A, for numerator and denominator each.
 * p_j rounded to 16 bits before the product (16-bit types): u A.
-* The result's own rounding: u |o| (plus half of fp16's smallest step).
+* The result's own rounding: u |o|, plus half of fp16's smallest step, and 2^-126
+  for bf16 and fp32: results below the smallest normal number may be flushed.
 """
 import math
 
@@ -60,7 +61,7 @@ def attention(q, k_cache, v_cache, block_tables, context_lens, cu, *, window=Non
     dt = q.dtype
     u = torch.finfo(dt).eps / 2
     u32 = 2.0 ** -24
-    floor = 2.0 ** -25 if dt == torch.float16 else 0.0
+    floor = 2.0 ** (-25 if dt == torch.float16 else -126)
     o, tol = torch.full((2, T, Hq, D), math.nan, dtype=torch.float64)
     lse, ltol = torch.full((2, Hq, T), math.nan, dtype=torch.float64)
     for s, ln in enumerate(context_lens.tolist()):

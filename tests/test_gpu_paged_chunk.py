@@ -44,7 +44,12 @@ def _check(b, window=None, sinks=0, impl=_lib.IMPL_AUTO, **kw):
     return out, lse
 
 
-IMPLS = {"auto": _lib.IMPL_AUTO, "simt": _lib.IMPL_SIMT}
+IMPLS = {"auto": _lib.IMPL_AUTO, "simt": _lib.IMPL_SIMT, "rows": _lib.IMPL_ROWS}
+
+
+def _skip_if_not_served(impl, dtype):
+    if impl == "rows" and dtype == F32:
+        pytest.skip("the few-rows kernel serves 16-bit types")
 LENS = [  # cached tokens, new tokens
     ([1], [1]),
     ([40, 17, 1, 0, 16], [3, 17, 1, 0, 16]),            # whole prompts, an empty sequence
@@ -60,6 +65,7 @@ LENS = [  # cached tokens, new tokens
 @pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64), (F32, 64)])
 @pytest.mark.parametrize("lens,new", LENS)
 def test_lengths(lens, new, dtype, D, quantised, impl):
+    _skip_if_not_served(impl, dtype)
     _check(R.build(lens, new, 2, 1, D, 16, dtype, quantised=quantised), impl=IMPLS[impl])
 
 
@@ -68,6 +74,7 @@ def test_lengths(lens, new, dtype, D, quantised, impl):
                                           (2 ** 40, 2 ** 40)])
 @pytest.mark.parametrize("dtype,quantised", [(BF16, False), (F16, True), (F32, False)])
 def test_windows(window, sinks, dtype, quantised, impl):
+    _skip_if_not_served(impl, dtype)
     b = R.build([9, 300, 1025, 130], [9, 140, 70, 1], 2, 2, 64, 16, dtype, quantised=quantised, seed=3)
     _check(b, window, sinks, IMPLS[impl])
 
@@ -183,6 +190,28 @@ def test_strided_q_and_out(new, quantised):
                               b["most"], k_scale=c["k_scale"], v_scale=c["v_scale"], out=out)
         R.check(out, want[0], want[1])
         assert bool((buf[:, H] == 2).all()) and bool((buf[:, :, off + D:] == 2).all()) and bool((buf[:, :, :off] == 2).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 12])
+def test_unequal_scales(new, D):
+    """Quantised rows whose scales span 2^-126 to 2^100: a bf16 cache with rows of zeros and of very small and
+    large V beside ordinary ones, and q rows of very different size."""
+    b = R.build([200, 300], [new, new], 2, 1, D, 16, BF16, seed=41)
+    g = torch.Generator().manual_seed(42)
+    shape = b["v_cache"].shape[:3]
+    pick = torch.randint(0, 6, shape, generator=g)
+    size = torch.tensor([1.0, 1.0, 0.0, 2.0 ** -40, 2.0 ** -110, 2.0 ** 20])[pick][..., None]
+    k = torch.randn(*b["k_cache"].shape, generator=g) * torch.exp(torch.randn(*shape, 1, generator=g))
+    (kq, ks), (vq, vs) = (R.quantise(x.to(BF16)) for x in (k, torch.randn(*b["v_cache"].shape, generator=g) * size))
+    b |= {"k_cache": kq.float().to(torch.float8_e4m3fn), "v_cache": vq.float().to(torch.float8_e4m3fn),
+          "k_scale": ks.float().to(torch.float8_e8m0fnu), "v_scale": vs.float().to(torch.float8_e8m0fnu)}
+    b["q"] *= torch.exp2(torch.arange(2 * new) * 6.0 - 60).to(BF16)[:, None, None].clamp(max=4)
+    _check(b)
+    _check(b, impl=_lib.IMPL_SIMT)
+    # every V row tiny: the result is as small, not zero
+    b["v_scale"].view(torch.uint8).fill_(20)
+    _check(b)
 
 
 def test_scale_argument():
