@@ -237,61 +237,80 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
 }
 
 // ----------------------------------------------------------------- combine --
-// One warp per (row, head): the grid is (row, head) pairs of the longest
-// sequence by sequences, so no row has to look its sequence up.
+// One CTA per (row, head): the grid is (row, head) pairs of the longest
+// sequence by sequences, so no row has to look its sequence up. Its 4 warps
+// take the chunks in turn (4 of them in flight per warp: a few hundred chunks
+// would otherwise be as many dependent trips to L2), then join.
 constexpr int C_WARPS = 4;
 
-template <typename T>
+template <typename T, int DC>
 __global__ void __launch_bounds__(C_WARPS * 32)
 paged_combine_kernel(const Params p, int R, int tk) {
   allow_dependents();
   wait_prerequisites();
+  __shared__ float sm[C_WARPS][DC * 32];
   const Seq q = load_seq(p, blockIdx.y);
-  const int id = blockIdx.x * C_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int i = id / p.Hq, h = id % p.Hq;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i = blockIdx.x / p.Hq, h = blockIdx.x % p.Hq;
   if (i >= q.n) return;
   int pos_lo, pos_hi;
   tile_positions(p, q, (i * p.G + h % p.G) / R, R, pos_lo, pos_hi);
   const KeySpan span(p, q, pos_lo, pos_hi, tk);
   const int chunks = chunks_of(p, span.count(), tk);
-  if (chunks == 1) return;
+  if (chunks == 1) return;  // written directly
   const int row = q.row0 + i;
   const int64_t at = ((int64_t)row * p.Hq + h) * p.P;
-  float mx = -INFINITY;
-  bool nan = false;
+  float mx = -INFINITY, bad = 0.f;
   for (int c = lane; c < chunks; c += 32) {
     const float x = p.part_lse[at + c];
-    nan |= x != x;
+    if (x != x) bad = x;
     mx = fmaxf(mx, x);
   }
   mx = warp_max(mx);
-  nan = __any_sync(0xffffffffu, nan);
+  bad = warp_sum(bad);  // NaN when a chunk's is
   const float m_use = mx == -INFINITY ? 0.f : mx;
   float sum = 0.f;
   for (int c = lane; c < chunks; c += 32) sum += exp2f(p.part_lse[at + c] - m_use);
   sum = warp_sum(sum);
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  T* dst = static_cast<T*>(p.o) + (int64_t)row * p.so_t + (int64_t)h * p.so_h;
-  for (int d = lane; d < p.D; d += 32) {
-    float a = 0.f;
-    for (int c = 0; c < chunks; ++c)
-      a = fmaf(exp2f(p.part_lse[at + c] - m_use), p.part_o[(at + c) * p.D + d], a);
-    dst[d] = from_f<T>(nan ? __int_as_float(0x7fc00000) : a * inv);
+  float acc[DC];
+#pragma unroll
+  for (int d = 0; d < DC; ++d) acc[d] = 0.f;
+#pragma unroll 4
+  for (int c = warp; c < chunks; c += C_WARPS) {
+    const float w = exp2f(p.part_lse[at + c] - m_use);
+#pragma unroll
+    for (int d = 0; d < DC; ++d)
+      if (d * 32 + lane < p.D) acc[d] = fmaf(w, p.part_o[(at + c) * p.D + d * 32 + lane], acc[d]);
   }
-  if (p.lse != nullptr && lane == 0)
+#pragma unroll
+  for (int d = 0; d < DC; ++d) sm[warp][d * 32 + lane] = acc[d];
+  __syncthreads();
+  const float inv = (sum > 0.f ? 1.f / sum : 0.f) + bad;
+  T* dst = static_cast<T*>(p.o) + (int64_t)row * p.so_t + (int64_t)h * p.so_h;
+  for (int d = threadIdx.x; d < p.D; d += C_WARPS * 32) {
+    float a = 0.f;
+#pragma unroll
+    for (int w = 0; w < C_WARPS; ++w) a += sm[w][d];
+    dst[d] = from_f<T>(a * inv);
+  }
+  if (p.lse != nullptr && threadIdx.x == 0)
     p.lse[(int64_t)h * p.T + row] =
-        nan ? __int_as_float(0x7fc00000)
-            : (sum > 0.f ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY);
+        (sum > 0.f ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY) + bad;
 }
 
 int launch_combine(const Params& p, int rows_per_tile, int tk, int dtype, cudaStream_t st) {
-  const int64_t blocks = ((int64_t)p.max_q * p.Hq + C_WARPS - 1) / C_WARPS;
-  LSB_CHECK_ARG(blocks <= 0x7fffffff, "paged_attn: too many rows to combine");
+  const int64_t blocks = (int64_t)p.max_q * p.Hq;
   return LSB_DISPATCH_DTYPE(dtype, T, [&] {
-    LSB_CUDA_OK(launch_kernel(paged_combine_kernel<T>, dim3((unsigned)blocks, (unsigned)p.S),
-                              dim3(C_WARPS * 32), 0, st, p, rows_per_tile, tk),
-                "paged_attn combine");
-    return LSB_OK;
+    auto go = [&](auto dc) -> int {
+      LSB_CUDA_OK(launch_kernel(paged_combine_kernel<T, decltype(dc)::value>,
+                                dim3((unsigned)blocks, (unsigned)p.S), dim3(C_WARPS * 32), 0, st, p,
+                                rows_per_tile, tk),
+                  "paged_attn combine");
+      return LSB_OK;
+    };
+    if (p.D <= 64) return go(std::integral_constant<int, 2>{});
+    if (p.D <= 128) return go(std::integral_constant<int, 4>{});
+    return go(std::integral_constant<int, 8>{});
   });
 }
 
@@ -328,8 +347,8 @@ constexpr int64_t ROWS_MAX_PAIRS = 64;
 static Plan plan_rows(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t keys) {
   if (max_q * G > ROWS_MAX_PAIRS) return {1 << 30, 1};
   const int64_t tiles = S * Hkv * ((max_q * G + ROWS_R - 1) / ROWS_R);
-  const int64_t P = std::max<int64_t>(1, 12 * 148 / tiles);
-  int64_t chunk = std::min<int64_t>(512, ((keys + P - 1) / P + 127) / 128 * 128);
+  const int64_t P = std::max<int64_t>(1, 3 * 148 / tiles);
+  int64_t chunk = std::min<int64_t>(1024, ((keys + P - 1) / P + 127) / 128 * 128);
   chunk = std::max<int64_t>(chunk, (keys / std::max<int64_t>(64, P) + 127) / 128 * 128);
   return {(int)std::min<int64_t>(chunk, 1 << 30),
           (int)std::max<int64_t>(1, (keys + chunk - 1) / chunk)};

@@ -9,18 +9,21 @@
 // warp-level MMA is the right size here: tcgen05's 128-row tiles would stage
 // every key through shared memory for one row of use.
 //
-// K and V go from global memory straight into MMA fragments, the next group's
-// loads in flight while the current one is computed; no shared memory, no
-// barriers in the loop. What makes that possible is that the contraction's
-// index order is free as long as both operands agree on it:
-//  * S = Q K^T: lane (g, t) = (lane / 4, lane % 4) loads 16-byte runs of key g's
+// Each warp streams its groups through a ring of its own in shared memory
+// (cp.async, 16 bytes a lane: STAGES groups in flight cost no registers and no
+// barrier beyond the warp's), and reads MMA fragments from it. What makes
+// whole 16-byte reads into fragments is that a contraction's index order is
+// free as long as both operands agree on it:
+//  * S = Q K^T: lane (g, t) = (lane / 4, lane % 4) reads 16-byte runs of key g's
 //    row at dims (4 i + t) EK and uses their 4-element pieces as its slots of
 //    consecutive k steps; Q is laid out by the same rule, once.
 //  * O += P V: the score fragment's columns (keys 2t, 2t + 1 of each half
-//    group) are P's A-operand slots as they stand. Lane (g, t) loads those four
+//    group) are P's A-operand slots as they stand. Lane (g, t) reads those four
 //    keys' V at dims (8 i + g) EV and interleaves pairs of keys with byte
 //    permutes into B fragments; output column g of n-tile j is dim
 //    (8 i + g) EV + e, j = i EV + e.
+// Rows are stored with their 16-byte pieces permuted (Shape::at) so that both
+// kinds of read touch every bank once.
 //
 // e4m3 cache: bytes convert to fp16 in one instruction per pair (exactly; the
 // MMAs run in fp16), unscaled. K's power-of-two scale multiplies the score. V's
@@ -55,30 +58,47 @@ __device__ __forceinline__ void mma16816(float& c0, float& c1, float& c2, float&
                                          uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   if constexpr (F16)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(c0), "+f"(c1), "+f"(c2), "+f"(c3)
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// N words from global memory, read once (16 bytes a load where N allows).
+// N words from shared memory (8 or 16 bytes).
 template <int N>
 __device__ __forceinline__ void load_words(uint32_t (&w)[N], const void* p) {
   static_assert(N == 2 || N == 4, "8 or 16 bytes");
   if constexpr (N == 4) {
-    const uint4 x = __ldcs(static_cast<const uint4*>(p));
+    const uint4 x = *static_cast<const uint4*>(p);
     w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
   } else {
-    const uint2 x = __ldcs(static_cast<const uint2*>(p));
+    const uint2 x = *static_cast<const uint2*>(p);
     w[0] = x.x; w[1] = x.y;
   }
+}
+
+// 16 bytes (8: scales) from global to shared memory, zeros when !there.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(there ? 8 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <bool FP8, int D>
@@ -91,29 +111,35 @@ struct Shape {
   static constexpr int WV = EV * EB / 4;           // words per V load
   static constexpr int STEPS = D / 16;             // k steps of S
   static constexpr int NT = D / 8;                 // n-tiles of O
+  static constexpr int CPR = D * EB / 16;          // 16-byte pieces of a row: 4, 8 or 16
+  static constexpr int HALF = 8 * CPR;             // pieces of 8 keys
+  static constexpr int TILE = TK * CPR * 16;       // bytes of a group's K (and V)
+  // A stage: K, V, and for e4m3 the scales (16 of K, 16 of V).
+  static constexpr int STAGE = 2 * TILE + (FP8 ? 32 : 0);
+  // Groups in flight per warp, sized so that an SM holds about 190 KB of ring.
+  static constexpr int STAGES = FP8 ? 4 : (D == 64 ? 4 : 3);
+  static constexpr int CTAS = FP8 ? (D == 64 ? 5 : 3) : (D == 64 ? 3 : 2);
+  // Byte offset of piece c of key k's row in its tile.
+  static __device__ __forceinline__ int at(int k, int c) {
+    if constexpr (CPR == 4) {  // two rows to a 128-byte line
+      const int line = k >> 1;
+      return (line * 8 + ((((k & 1) << 2) | c) ^ ((line & 3) << 1))) * 16;
+    } else {
+      return (k * CPR + (c ^ ((((k >> 1) & 3) << 1) ^ ((k & 1) << 2)))) * 16;
+    }
+  }
 };
 
-// One group's operands as they arrive: K rows of keys g and 8 + g, V rows of
-// keys 2t, 2t + 1, 8 + 2t, 8 + 2t + 1, and the scales of those four keys.
-template <bool FP8, int D>
-struct Group {
-  using S = Shape<FP8, D>;
-  uint32_t k[2][S::NK][4];
-  uint32_t v[4][S::NV][S::WV];
-  uint16_t ks[2], vs[2];
-  int tok0;
-  int ids[2];  // page of each half, -1: no such page
-};
+// Dynamic shared memory of a CTA: the rings, which the merge reuses.
+template <bool FP8, int D, bool R8>
+constexpr int smem_bytes() {
+  const int ring = WARPS * Shape<FP8, D>::STAGES * Shape<FP8, D>::STAGE;
+  const int merge = WARPS * (R8 ? 8 : 16) * (D + 4 + 3) * 4;
+  return ring > merge ? ring : merge;
+}
 
 template <typename T, bool FP8, int D, bool R8>
-struct Occupancy {
-  // Resident CTAs the registers are budgeted for: two groups in flight take
-  // 64 (e4m3) or 128 registers, Q and O 48 (8 rows) or 96, at D = 128.
-  static constexpr int CTAS = D == 64 ? (FP8 && R8 ? 5 : 4) : (FP8 && R8 ? 3 : 2);
-};
-
-template <typename T, bool FP8, int D, bool R8>
-__global__ void __launch_bounds__(WARPS * 32, (Occupancy<T, FP8, D, R8>::CTAS))
+__global__ void __launch_bounds__(WARPS * 32, (Shape<FP8, D>::CTAS))
 paged_rows_kernel(const Params p) {
   allow_dependents();
   wait_prerequisites();
@@ -121,8 +147,11 @@ paged_rows_kernel(const Params p) {
   constexpr bool F16 = FP8 || std::is_same<T, __half>::value;  // MMA operand type
   constexpr int ROWS = R8 ? 8 : 16;
   constexpr int HALVES = R8 ? 1 : 2;
-  __shared__ float sm_acc[WARPS][ROWS][D];
-  __shared__ float sm_m[WARPS][ROWS], sm_l[WARPS][ROWS], sm_w[WARPS][ROWS];
+  extern __shared__ __align__(16) uint8_t smem[];
+  float(*sm_acc)[ROWS][D + 4] = reinterpret_cast<float(*)[ROWS][D + 4]>(smem);
+  float(*sm_m)[ROWS] = reinterpret_cast<float(*)[ROWS]>(smem + sizeof(float) * WARPS * ROWS * (D + 4));
+  float(*sm_l)[ROWS] = sm_m + WARPS;
+  float(*sm_w)[ROWS] = sm_l + WARPS;
 
   const int chunk = blockIdx.x % p.P, hk = blockIdx.x / p.P, tile = blockIdx.y, s = blockIdx.z;
   const Seq q = load_seq(p, s);
@@ -190,7 +219,8 @@ paged_rows_kernel(const Params p) {
   }
 
   // ------------------------------------------------------------- loads ----
-  // Page ids of this warp's next 16 groups, one half group per lane.
+  // Page ids of 16 of this warp's groups from v on, one half group per lane;
+  // -1: no such page.
   auto fetch_ids = [&](int v) -> int {
     const int vv = v + (lane >> 1) * WARPS;
     if (vv >= v1) return -1;
@@ -201,40 +231,33 @@ paged_rows_kernel(const Params p) {
   };
   const uint8_t* kc = static_cast<const uint8_t*>(p.k_cache);
   const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
-  auto load = [&](Group<FP8, D>& x, int v, int id0, int id1) {
-    x.tok0 = span.tile(v) * TK;
-    x.ids[0] = id0;
-    x.ids[1] = id1;
+  uint8_t* ring = smem + warp * (S::STAGES * S::STAGE);
+  // Copies the group at keys [tok0, tok0 + 16) into a stage. Missing pages and
+  // V rows that no row of the tile sees arrive as zeros, so what such cells
+  // hold never meets a weight of 0.
+  auto copy_group = [&](int stage, int tok0, int id0, int id1) {
+    const uint32_t dst = sm100::smem_u32(ring + stage * S::STAGE);
+    const bool whole = tok0 + TK - 1 <= pos_lo && tok0 + TK <= q.ctx && p.window == 0;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const int id = x.ids[hf];
-      if (id >= 0) {
-        const int64_t cell = ((int64_t)id * p.Hkv + hk) * bs + ((x.tok0 + 8 * hf) & (bs - 1));
-        const uint8_t* kr = kc + (cell + g) * (D * S::EB) + t * 16;
+      const int id = hf == 0 ? id0 : id1;
+      const bool there = id >= 0;
+      const int64_t cell =
+          there ? ((int64_t)id * p.Hkv + hk) * bs + ((tok0 + 8 * hf) & (bs - 1)) : 0;
+      const uint8_t* ks = kc + cell * (D * S::EB) + lane * 16;
+      const uint8_t* vs = vc + cell * (D * S::EB) + lane * 16;
 #pragma unroll
-        for (int i = 0; i < S::NK; ++i) load_words(x.k[hf][i], kr + i * 64);
-        const uint8_t* vr = vc + (cell + 2 * t) * (D * S::EB) + g * (S::EV * S::EB);
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < S::NV; ++i)
-            load_words(x.v[2 * hf + e][i], vr + e * (D * S::EB) + i * (8 * S::EV * S::EB));
-        if constexpr (FP8) {
-          x.ks[hf] = *reinterpret_cast<const uint16_t*>(p.k_scale + cell + 2 * t);
-          x.vs[hf] = *reinterpret_cast<const uint16_t*>(p.v_scale + cell + 2 * t);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < S::NK; ++i)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) x.k[hf][i][w] = 0u;
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < S::NV; ++i)
-#pragma unroll
-            for (int w = 0; w < S::WV; ++w) x.v[2 * hf + e][i][w] = 0u;
-        x.ks[hf] = x.vs[hf] = 0x7f7f;
+      for (int i = 0; i < S::HALF / 32; ++i) {
+        const int piece = i * 32 + lane, k = hf * 8 + piece / S::CPR, c = piece % S::CPR;
+        const uint32_t to = dst + S::at(k, c);
+        copy16(to, ks + i * 512, there);
+        copy16(to + S::TILE, vs + i * 512,
+               there && (whole || seen_by_any(p, pos_lo, pos_hi, q.ctx, tok0 + k)));
+      }
+      if constexpr (FP8) {
+        if (lane < 2)
+          copy8(dst + 2 * S::TILE + lane * 16 + hf * 8, (lane == 0 ? p.k_scale : p.v_scale) + cell,
+                there);
       }
     }
   };
@@ -251,64 +274,73 @@ paged_rows_kernel(const Params p) {
 #pragma unroll
     for (int e = 0; e < 2 * HALVES; ++e) acc[j][e] = 0.f;
 
-  auto compute = [&](Group<FP8, D>& x) {
-    float sc[2][4];
+  auto scores = [&](const uint8_t* kt, float (&sc)[2][4]) {
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
 #pragma unroll
-    for (int st = 0; st < S::STEPS; ++st) {
-      const int i = st / (S::EK / 4), w = st % (S::EK / 4);
+    for (int i = 0; i < S::NK; ++i) {
+      uint32_t k[2][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        uint32_t b0, b1;
-        if constexpr (FP8) {
-          b0 = cvt_e4m3x2_f16x2((uint16_t)(x.k[n][i][w] & 0xffff));
-          b1 = cvt_e4m3x2_f16x2((uint16_t)(x.k[n][i][w] >> 16));
-        } else {
-          b0 = x.k[n][i][2 * w];
-          b1 = x.k[n][i][2 * w + 1];
+      for (int n = 0; n < 2; ++n) load_words(k[n], kt + S::at(8 * n + g, 4 * i + t));
+#pragma unroll
+      for (int w = 0; w < S::EK / 4; ++w) {
+        const int st = i * (S::EK / 4) + w;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          uint32_t b0, b1;
+          if constexpr (FP8) {
+            b0 = cvt_e4m3x2_f16x2((uint16_t)(k[n][w] & 0xffff));
+            b1 = cvt_e4m3x2_f16x2((uint16_t)(k[n][w] >> 16));
+          } else {
+            b0 = k[n][2 * w];
+            b1 = k[n][2 * w + 1];
+          }
+          mma16816<F16>(sc[n][0], sc[n][1], sc[n][2], sc[n][3], qa[0][st][0],
+                        R8 ? 0u : qa[HALVES - 1][st][0], qa[0][st][1],
+                        R8 ? 0u : qa[HALVES - 1][st][1], b0, b1);
         }
-        mma16816<F16>(sc[n][0], sc[n][1], sc[n][2], sc[n][3], qa[0][st][0],
-                      R8 ? 0u : qa[HALVES - 1][st][0], qa[0][st][1],
-                      R8 ? 0u : qa[HALVES - 1][st][1], b0, b1);
       }
     }
-    // Scores in log2 units; keys that a row does not see go to -inf.
-    const int last = x.tok0 + TK - 1;
-    const bool whole = last <= pos_lo && last < q.ctx && x.ids[0] >= 0 && x.ids[1] >= 0 &&
-                       (p.window == 0 || pos_hi - x.tok0 < p.window || last < p.sinks);
+  };
+  // Weights of the group's keys as A fragments [row half][half group]. Scores
+  // go to log2 units, to -inf for keys that a row does not see.
+  auto weights = [&](const uint8_t* scales, float (&sc)[2][4], int tok0, const int (&ids)[2],
+                     uint32_t (&pa)[HALVES][2]) {
+    const int last = tok0 + TK - 1;
+    const bool whole = last <= pos_lo && last < q.ctx && ids[0] >= 0 && ids[1] >= 0 &&
+                       (p.window == 0 || pos_hi - tok0 < p.window || last < p.sinks);
     float ev[2][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 2; ++n) {
+      uint32_t ks = 0, vs = 0;
+      if constexpr (FP8) {
+        ks = *reinterpret_cast<const uint16_t*>(scales + 8 * n + 2 * t);
+        vs = *reinterpret_cast<const uint16_t*>(scales + 16 + 8 * n + 2 * t);
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float f = 1.f;
         if constexpr (FP8) {
-          f = e8m0_to_float((x.ks[n] >> (8 * e)) & 0xff);
-          const int b = (x.vs[n] >> (8 * e)) & 0xff;
+          f = e8m0_to_float((ks >> (8 * e)) & 0xff);
+          const int b = (vs >> (8 * e)) & 0xff;
           ev[n][e] = b == 255 ? __int_as_float(0x7fc00000) : (float)(b - 127);
         }
 #pragma unroll
         for (int hf = 0; hf < HALVES; ++hf) sc[n][2 * hf + e] *= fac[hf] * f;
       }
+    }
     if (!whole) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int j = x.tok0 + 8 * n + 2 * t + e;
+          const int j = tok0 + 8 * n + 2 * t + e;
 #pragma unroll
           for (int hf = 0; hf < HALVES; ++hf)
-            if (x.ids[n] < 0 || !sees(p, pos[hf], q.ctx, j)) sc[n][2 * hf + e] = -INFINITY;
-          if (!seen_by_any(p, pos_lo, pos_hi, q.ctx, j)) {
-            ev[n][e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < S::NV; ++i)
-#pragma unroll
-              for (int w = 0; w < S::WV; ++w) x.v[2 * n + e][i][w] = 0u;
-          }
+            if (ids[n] < 0 || !sees(p, pos[hf], q.ctx, j)) sc[n][2 * hf + e] = -INFINITY;
+          if (FP8 && !seen_by_any(p, pos_lo, pos_hi, q.ctx, j)) ev[n][e] = 0.f;
         }
     }
     bool raise = false;
@@ -350,7 +382,6 @@ paged_rows_kernel(const Params p) {
         }
       }
     }
-    uint32_t pa[HALVES][2];  // P as A fragments: [row half][half group]
 #pragma unroll
     for (int hf = 0; hf < HALVES; ++hf) {
       const float mm = m[hf] == -INFINITY ? 0.f : m[hf] - LIFT;
@@ -366,6 +397,8 @@ paged_rows_kernel(const Params p) {
           pa[hf][n] = F16 ? sm100::pack_f16(p0, p1) : sm100::pack_bf16(p0, p1);
       }
     }
+  };
+  auto weigh_v = [&](const uint8_t* vt, const uint32_t (&pa)[HALVES][2]) {
     auto pv = [&](int j, uint32_t b0, uint32_t b1) {
       float z0 = 0.f, z1 = 0.f;  // rows 8-15 of an 8-row tile
       mma16816<F16>(acc[j][0], acc[j][1], R8 ? z0 : acc[j][2 * HALVES - 2],
@@ -373,10 +406,15 @@ paged_rows_kernel(const Params p) {
                     pa[0][1], R8 ? 0u : pa[HALVES - 1][1], b0, b1);
     };
 #pragma unroll
-    for (int i = 0; i < S::NV; ++i)
+    for (int i = 0; i < S::NV; ++i) {
+      uint32_t vw[4][S::WV];  // keys 2t, 2t + 1, 8 + 2t, 8 + 2t + 1
+      const int byte = (8 * i + g) * (S::EV * S::EB);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        load_words(vw[e], vt + S::at((e >> 1) * 8 + 2 * t + (e & 1), byte / 16) + byte % 16);
 #pragma unroll
       for (int w = 0; w < S::WV; ++w) {
-        const uint32_t a = x.v[0][i][w], b = x.v[1][i][w], c = x.v[2][i][w], d = x.v[3][i][w];
+        const uint32_t a = vw[0][w], b = vw[1][w], c = vw[2][w], d = vw[3][w];
         if constexpr (FP8) {
           const int j = i * S::EV + 4 * w;
           const uint32_t lo0 = __byte_perm(a, b, 0x5140), lo1 = __byte_perm(c, d, 0x5140);
@@ -391,43 +429,55 @@ paged_rows_kernel(const Params p) {
           pv(j + 1, __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
         }
       }
+    }
   };
 
   {
-    int v = v0 + warp;
-    int ids = fetch_ids(v), at = 0;
-    auto next_ids = [&](int vv, int& a, int& b) {  // ids of group vv, the at-th of the fetched 16
-      if (at == 16) {
-        ids = fetch_ids(vv);
-        at = 0;
+    // Group n of this warp is v0 + warp + n WARPS and sits in stage n % STAGES.
+    constexpr int AHEAD = S::STAGES - 1;
+    const int mine = v1 - v0 > warp ? (v1 - v0 - warp + WARPS - 1) / WARPS : 0;
+    const int first = v0 + warp;
+    int near = fetch_ids(first), far = fetch_ids(first + 16 * WARPS);
+    auto copy_next = [&](int n) {  // called for n = 0, 1, 2, ... in turn
+      if (n > 0 && n % 16 == 0) {
+        near = far;
+        far = fetch_ids(first + (n + 16) * WARPS);
       }
-      a = __shfl_sync(0xffffffffu, ids, 2 * at);
-      b = __shfl_sync(0xffffffffu, ids, 2 * at + 1);
-      ++at;
+      const int a = __shfl_sync(0xffffffffu, near, 2 * (n % 16));
+      const int b = __shfl_sync(0xffffffffu, near, 2 * (n % 16) + 1);
+      if (n < mine) copy_group(n % S::STAGES, span.tile(first + n * WARPS) * TK, a, b);
+      copies_commit();  // a group of copies per n, empty past the end
+      return (a >= 0 ? 1 : 0) | (b >= 0 ? 2 : 0);
     };
-    int a = -1, b = -1;
-    Group<FP8, D> cur, nxt;
-    if (v < v1) {
-      next_ids(v, a, b);
-      load(cur, v, a, b);
+    uint32_t there = 0;  // two bits per group in flight: which halves have a page
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) there |= copy_next(n) << (2 * n);
+    for (int n = 0; n < mine; ++n) {
+      copies_wait<AHEAD - 1>();  // this lane's copies of group n are in
+      __syncwarp();              // every lane's are, and group n - 1 has been read by all
+      there |= copy_next(n + AHEAD) << (2 * AHEAD);
+      const uint8_t* st = ring + (n % S::STAGES) * S::STAGE;
+      const int ids[2] = {(there & 1) ? 0 : -1, (there & 2) ? 0 : -1};
+      there >>= 2;
+      const int tok0 = span.tile(first + n * WARPS) * TK;
+      float sc[2][4];
+      scores(st, sc);
+      uint32_t pa[HALVES][2];
+      weights(st + 2 * S::TILE, sc, tok0, ids, pa);
+      weigh_v(st + S::TILE, pa);
     }
-    for (; v < v1; v += WARPS) {
-      const bool more = v + WARPS < v1;
-      if (more) {
-        next_ids(v + WARPS, a, b);
-        load(nxt, v + WARPS, a, b);
-      }
-      compute(cur);
-      if (more) cur = nxt;
-    }
+    copies_wait<0>();
   }
+  __syncthreads();  // the merge reuses the rings
 
   // ------------------------------------------------------------- merge ----
 #pragma unroll
   for (int hf = 0; hf < HALVES; ++hf) {
     l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
     l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+    __syncwarp();
     const int r = hf * 8 + g;
+    if (tile * 16 + r >= pairs) continue;
     if (t == 0) {
       sm_m[warp][r] = m[hf];
       sm_l[warp][r] = l[hf];
@@ -483,17 +533,22 @@ paged_rows_kernel(const Params p) {
   }
 }
 
+template <typename T, bool FP8, int D, bool R8>
+static int launch_tile(const Params& p, dim3 grid, cudaStream_t st) {
+  constexpr int smem = smem_bytes<FP8, D, R8>();
+  auto kern = paged_rows_kernel<T, FP8, D, R8>;
+  static SmemLimit limit;
+  if (int rc = limit.ensure(kern, smem, "paged_attn smem attribute")) return rc;
+  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(WARPS * 32), smem, st, p), "paged_attn");
+  return LSB_OK;
+}
+
 template <typename T, bool FP8, int D>
 static int launch(const Params& p, cudaStream_t st) {
   const int64_t pairs = (int64_t)p.max_q * p.G;
   const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)((pairs + 15) / 16), (unsigned)p.S);
-  if (pairs <= 8)
-    LSB_CUDA_OK(launch_kernel(paged_rows_kernel<T, FP8, D, true>, grid, dim3(WARPS * 32), 0, st, p),
-                "paged_attn");
-  else
-    LSB_CUDA_OK(launch_kernel(paged_rows_kernel<T, FP8, D, false>, grid, dim3(WARPS * 32), 0, st, p),
-                "paged_attn");
-  return LSB_OK;
+  return pairs <= 8 ? launch_tile<T, FP8, D, true>(p, grid, st)
+                    : launch_tile<T, FP8, D, false>(p, grid, st);
 }
 
 }  // namespace rows
@@ -501,12 +556,12 @@ static int launch(const Params& p, cudaStream_t st) {
 bool rows_eligible(const Params& p, int dtype, bool kv_fp8) {
   if (dtype != LSB_DTYPE_BF16 && dtype != LSB_DTYPE_F16) return false;
   if ((p.D != 64 && p.D != 128) || p.bs_log2 < 3) return false;
-  // q rows are read in 8-byte pieces, the cache in 8- and 16-byte ones, the
-  // scales in pairs.
+  // q rows are read in 8-byte pieces, the cache in 16-byte ones, the scales of
+  // 8 keys at a time.
   auto at = [](const void* x, uintptr_t a) { return (reinterpret_cast<uintptr_t>(x) & (a - 1)) == 0; };
   if (!at(p.q, 8) || p.sq_t % 4 != 0 || p.sq_h % 4 != 0) return false;
   if (!at(p.k_cache, 16) || !at(p.v_cache, 16)) return false;
-  if (kv_fp8 && (!at(p.k_scale, 2) || !at(p.v_scale, 2))) return false;
+  if (kv_fp8 && (!at(p.k_scale, 8) || !at(p.v_scale, 8))) return false;
   return ((int64_t)p.max_q * p.G + 15) / 16 <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff;
 }
 
