@@ -346,7 +346,8 @@ constexpr int64_t ROWS_MAX_PAIRS = 64;
 
 static Plan plan_rows(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t keys) {
   if (max_q * G > ROWS_MAX_PAIRS) return {1 << 30, 1};
-  const int64_t tiles = S * Hkv * ((max_q * G + ROWS_R - 1) / ROWS_R);
+  const int64_t R = rows_tile(max_q * G);
+  const int64_t tiles = S * Hkv * ((max_q * G + R - 1) / R);
   const int64_t P = std::max<int64_t>(1, 3 * 148 / tiles);
   int64_t chunk = std::min<int64_t>(1024, ((keys + P - 1) / P + 127) / 128 * 128);
   chunk = std::max<int64_t>(chunk, (keys / std::max<int64_t>(64, P) + 127) / 128 * 128);
@@ -465,5 +466,5 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
   cudaStream_t st = (cudaStream_t)stream;
   const int rc = rows ? launch_rows(p, dtype, fp8, st) : launch_simt(p, dtype, fp8, st);
   if (rc != LSB_OK || p.P == 1) return rc;
-  return rows ? launch_combine(p, ROWS_R, ROWS_TK, dtype, st) : launch_combine(p, SR, STK, dtype, st);
+  return rows ? launch_combine(p, rows_tile((int64_t)max_seqlen_q * p.G), ROWS_TK, dtype, st) : launch_combine(p, SR, STK, dtype, st);
 }

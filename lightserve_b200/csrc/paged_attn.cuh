@@ -129,7 +129,11 @@ int launch_combine(const Params& p, int rows_per_tile, int tk, int dtype, cudaSt
 // Each kernel's launcher. `kv_fp8`: the cache holds e4m3.
 int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 
-constexpr int ROWS_R = 16, ROWS_TK = 16;  // paged_attn_rows.cu's query tile and key group
+// paged_attn_rows.cu's key group, and the pairs of its query tile: 8, 16 or 24,
+// the fewest that hold a sequence's (more pairs take several tiles, each of
+// which reads the cache again).
+constexpr int ROWS_TK = 16;
+inline int rows_tile(int64_t pairs) { return pairs <= 8 ? 8 : pairs <= 16 ? 16 : 24; }
 bool rows_eligible(const Params& p, int dtype, bool kv_fp8);
 int launch_rows(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 
