@@ -289,7 +289,7 @@ LSB_API int lsb_rope_kv_quantize(const void* qkv, int64_t s_s, int64_t s_part, i
  * window > 0, p - j < window or j < num_sinks. A row that sees none gives 0.
  * lse (optional): fp32 [Hq, total_q], natural log (-inf when no key is seen).
  * Rows of no sequence, or past max_seqlen_q of theirs, are left as they were.
- * workspace: >= lsb_paged_attn_workspace_size bytes, 16-byte aligned (may be
+ * workspace: >= lsb_paged_attn_workspace_size bytes, 32-byte aligned (may be
  * NULL when that size is 0); calls that run at the same time need their own.
  * impl: LSB_IMPL_AUTO, or one of the kernels (error when it does not serve
  * the call).

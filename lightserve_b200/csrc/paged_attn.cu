@@ -355,6 +355,14 @@ static Plan plan_rows(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t 
           (int)std::max<int64_t>(1, (keys + chunk - 1) / chunk)};
 }
 
+// Pairs of a CTA of the tcgen05 kernel: two query tiles.
+static int64_t tc_pairs(int64_t G) { return 2 * std::max<int64_t>(1, 128 / G) * G; }
+
+static Plan plan_tc(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t keys) {
+  const int64_t items = S * Hkv * ((max_q * G + tc_pairs(G) - 1) / tc_pairs(G));
+  return plan_split(items, keys, 148, 512);
+}
+
 }  // namespace pa
 }  // namespace lsb
 
@@ -371,7 +379,8 @@ extern "C" int64_t lsb_paged_attn_workspace_size(int64_t num_seqs, int64_t total
       max_visible(max_seqlen_q, max_blocks_per_seq * block_size, window, num_sinks);
   const int64_t G = Hq / Hkv;
   const int64_t P = std::max(plan_simt(num_seqs, max_seqlen_q, Hkv, G, keys).P,
-                             plan_rows(num_seqs, max_seqlen_q, Hkv, G, keys).P);
+                             std::max(plan_rows(num_seqs, max_seqlen_q, Hkv, G, keys).P,
+                                      plan_tc(num_seqs, max_seqlen_q, Hkv, G, keys).P));
   if (P <= 1) return 0;
   return lsb::align256(4 * total_q * Hq * P) + 4 * total_q * Hq * P * D;
 }
@@ -422,7 +431,8 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
     lsb::set_error("paged_attn: head dim %lld above 256", (long long)D);
     return LSB_ERR_UNSUPPORTED;
   }
-  LSB_CHECK_ARG(impl == LSB_IMPL_AUTO || impl == LSB_IMPL_SIMT || impl == LSB_IMPL_ROWS,
+  LSB_CHECK_ARG(impl == LSB_IMPL_AUTO || impl == LSB_IMPL_SIMT || impl == LSB_IMPL_ROWS ||
+                    impl == LSB_IMPL_TCGEN05,
                 "paged_attn: bad impl %d", impl);
 
   Params p = {};
@@ -441,30 +451,53 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
   p.sinks = (int)std::min<int64_t>(num_sinks, kMax);
   p.scale_log2 = scale * LOG2E;
   const int64_t keys = max_visible(max_seqlen_q, max_blocks_per_seq * block_size, p.window, p.sinks);
-  Plan plan = plan_rows(num_seqs, max_seqlen_q, Hkv, p.G, keys);
-  p.P = plan.P;
-  const bool rows_ok = rows_eligible(p, dtype, fp8);
+  const Plan rows_plan = plan_rows(num_seqs, max_seqlen_q, Hkv, p.G, keys);
+  const Plan tc_plan = plan_tc(num_seqs, max_seqlen_q, Hkv, p.G, keys);
+  p.P = std::max(rows_plan.P, tc_plan.P);  // (the grids' limits)
+  const bool rows_ok = rows_eligible(p, dtype, fp8), tc_ok = tc_eligible(p, dtype, fp8);
   LSB_CHECK_ARG(impl != LSB_IMPL_ROWS || rows_ok,
                 "paged_attn: the few-rows kernel needs bf16/fp16, D in {64,128}, pages of 8 keys or "
                 "more, q strides that are multiples of 4 elements and 16-byte aligned caches");
-  const bool rows = impl == LSB_IMPL_ROWS ||
-                    (impl == LSB_IMPL_AUTO && rows_ok && max_seqlen_q * p.G <= ROWS_MAX_PAIRS);
-  if (!rows) plan = plan_simt(num_seqs, max_seqlen_q, Hkv, p.G, keys);
+  LSB_CHECK_ARG(impl != LSB_IMPL_TCGEN05 || tc_ok,
+                "paged_attn: the tcgen05 kernel needs bf16/fp16, D in {64,128}, pages of 8 keys or "
+                "more, a positive scale, at most 128 heads per group and 16-byte aligned tensors "
+                "and strides");
+  // Few rows: bandwidth decides, and the few-rows kernel reads the cache at
+  // full rate. Many: the tensor cores. Tensors whose alignment rules a kernel
+  // out take the other one, then the CUDA cores.
+  if (impl == LSB_IMPL_AUTO) {
+    const bool few = max_seqlen_q * p.G <= ROWS_MAX_PAIRS;
+    impl = rows_ok && (few || !tc_ok) ? LSB_IMPL_ROWS : tc_ok ? LSB_IMPL_TCGEN05 : LSB_IMPL_SIMT;
+  }
+  const Plan plan = impl == LSB_IMPL_ROWS      ? rows_plan
+                    : impl == LSB_IMPL_TCGEN05 ? tc_plan
+                                               : plan_simt(num_seqs, max_seqlen_q, Hkv, p.G, keys);
   p.chunk = plan.chunk;
   p.P = plan.P;
   if (p.P > 1) {
     const int64_t need = lsb_paged_attn_workspace_size(num_seqs, total_q, max_seqlen_q, Hq, Hkv, D,
                                                        max_blocks_per_seq, block_size, window,
                                                        num_sinks);
-    LSB_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && lsb::aligned16(workspace),
-                  "paged_attn: workspace of %lld bytes (16-byte aligned) required, got %lld",
+    LSB_CHECK_ARG(workspace != nullptr && workspace_bytes >= need &&
+                      (reinterpret_cast<uintptr_t>(workspace) & 31) == 0,
+                  "paged_attn: workspace of %lld bytes (32-byte aligned) required, got %lld",
                   (long long)need, (long long)workspace_bytes);
     p.part_lse = static_cast<float*>(workspace);
     p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                         lsb::align256(4 * total_q * Hq * p.P));
   }
   cudaStream_t st = (cudaStream_t)stream;
-  const int rc = rows ? launch_rows(p, dtype, fp8, st) : launch_simt(p, dtype, fp8, st);
+  if (impl == LSB_IMPL_ROWS) {
+    const int rc = launch_rows(p, dtype, fp8, st);
+    if (rc != LSB_OK || p.P == 1) return rc;
+    return launch_combine(p, rows_tile(max_seqlen_q * p.G), ROWS_TK, dtype, st);
+  }
+  if (impl == LSB_IMPL_TCGEN05) {
+    const int rc = launch_tc(p, dtype, fp8, st);
+    if (rc != LSB_OK || p.P == 1) return rc;
+    return launch_combine(p, (int)tc_pairs(p.G), TC_TK, dtype, st);
+  }
+  const int rc = launch_simt(p, dtype, fp8, st);
   if (rc != LSB_OK || p.P == 1) return rc;
-  return rows ? launch_combine(p, rows_tile((int64_t)max_seqlen_q * p.G), ROWS_TK, dtype, st) : launch_combine(p, SR, STK, dtype, st);
+  return launch_combine(p, SR, STK, dtype, st);
 }

@@ -78,6 +78,7 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int s) {
 // s_tiles tiles from key 0 on, then the tiles [lo, hi).
 struct KeySpan {
   int s_tiles, lo, hi;
+  KeySpan() = default;
   __device__ __forceinline__ KeySpan(const Params& p, const Seq& q, int pos_lo, int pos_hi, int tk) {
     const int end = max(min(q.ctx, pos_hi + 1), 0);  // keys from here on are seen by none
     hi = (end + tk - 1) / tk;
@@ -134,6 +135,9 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 // which reads the cache again).
 constexpr int ROWS_TK = 16;
 inline int rows_tile(int64_t pairs) { return pairs <= 8 ? 8 : pairs <= 16 ? 16 : 24; }
+constexpr int TC_TK = 128;  // paged_attn_sm100.cu's key tile; a query tile holds (128 / G) G pairs
+bool tc_eligible(const Params& p, int dtype, bool kv_fp8);
+int launch_tc(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 bool rows_eligible(const Params& p, int dtype, bool kv_fp8);
 int launch_rows(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 

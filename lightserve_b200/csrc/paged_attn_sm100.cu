@@ -1,0 +1,664 @@
+// Paged attention for many rows per sequence (chunked prefill) on the
+// 5th-generation tensor cores.
+//
+// One CTA: two query tiles of up to 128 pairs (row, head of the group) of one
+// (sequence, cache head), and one chunk of the keys they see, in tiles of 128.
+// The inner loop is the one of the contiguous forward kernel: S_t = Q_t K^T
+// (tcgen05 SS, fp32 in TMEM), softmax with one thread per row (TMEM lane) and a
+// conditional rescale, P packed to 16 bits over S in two halves, O_t += P_t V
+// (TS), the two query tiles' MMA batches and softmaxes alternating. What
+// differs is where K and V come from and which keys count:
+//  * 16-bit cache: one TMA box per page, head and 64-column half. A page's rows
+//    land where the 128-byte swizzle wants them, since boxes start at multiples
+//    of 8 rows, so a tile of pages looks like a tile of one tensor. Pages that do
+//    not exist, or that no row sees, are fetched at an out-of-range block: zeros.
+//  * e4m3 cache: a converter warpgroup reads the rows (16 bytes a thread, one
+//    tile ahead in registers), multiplies by the row's power of two in fp32 and
+//    rounds to q's type, which is exact in bf16 (and in fp16 within its range),
+//    and writes the swizzled tile. Converting in the MMA's shadow costs no time
+//    on the S -> softmax -> P chain that bounds the kernel.
+//  * V rows that no row of the item sees (past the context, between sinks and
+//    window) are zeroed in shared memory, so that what such cells hold never
+//    meets a weight of 0; the tiles that need it are the ends of a span.
+//  * A pair's heads of one group share the K/V tiles: row r of a tile is
+//    token r / G, head r % G.
+//
+// Warps: 0 loads (Q; K, V of a 16-bit cache), 1 issues MMAs and owns TMEM,
+// 4-7 and 8-11 softmax of query tile 0 and 1, 12-15 convert (e4m3 only).
+// TMEM: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512) columns. Every
+// mbarrier wait is bounded; on a timeout the error word is set, the role ends,
+// TMEM is freed and the CTA exits.
+#include "paged_attn.cuh"
+#include "sm100.cuh"
+#include "tma_host.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace lsb {
+namespace pa {
+namespace tc {
+
+using namespace sm100;
+
+constexpr int BM = 128;
+constexpr int BN = TC_TK;
+constexpr int TILES = 2;
+constexpr int NS = 2;  // K/V ring stages
+constexpr int CHUNK_BYTES = 128 * 128;  // [128 rows][64 columns] of 16 bits
+constexpr float RESCALE_THRESHOLD = 8.0f;
+
+template <int D>
+struct Smem {
+  static constexpr int KC = D / 64;
+  static constexpr int Q_OFF = 0;
+  static constexpr int K_OFF = Q_OFF + TILES * KC * CHUNK_BYTES;
+  static constexpr int V_OFF = K_OFF + NS * KC * CHUNK_BYTES;
+  static constexpr int BAR_OFF = V_OFF + NS * KC * CHUNK_BYTES;
+  // q_full[2], k_full[NS], v_full[NS], kv_empty[NS], s_full[2], p_full[2][2], pv_done[2], edge
+  static constexpr int NBAR = TILES + 3 * NS + 4 * TILES + 1;
+  static constexpr int TMEM_SLOT_OFF = BAR_OFF + NBAR * 8;
+  static constexpr int PAGES_OFF = TMEM_SLOT_OFF + 16;  // [NS] bit per 8 keys: page there
+  static constexpr int BYTES = PAGES_OFF + NS * 4;
+  static constexpr int ALLOC = BYTES + 1024;  // slack for 1024-byte alignment
+};
+
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+__device__ __forceinline__ void st_global_v8(void* dst, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]),
+               "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ float row_max(const uint32_t (&sr)[4][32]) {
+  float mx8[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) mx8[u] = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int cc = 0; cc < 32; cc += 2)
+      mx8[(cc >> 1) & 7] = max3f(mx8[(cc >> 1) & 7], __uint_as_float(sr[i][cc]),
+                                 __uint_as_float(sr[i][cc + 1]));
+  return fmaxf(max3f(mx8[0], mx8[1], mx8[2]),
+               max3f(max3f(mx8[3], mx8[4], mx8[5]), mx8[6], mx8[7]));
+}
+
+// Everything a role needs to know about the CTA's work; each thread derives
+// it from the lengths in device memory.
+struct Item {
+  Seq q;
+  int hk, pairs, R;         // R: pairs per query tile
+  int c0;                   // the item's first query tile
+  int pos_lo, pos_hi;       // positions of its rows
+  KeySpan span;
+  int v0, nkv, nkv_t[TILES];  // first span tile, tiles visited by the item and by each query tile
+  int chunk, chunks;
+};
+
+// False: this CTA has nothing to do.
+__device__ __forceinline__ bool make_item(const Params& p, Item& w) {
+  w.q = load_seq(p, blockIdx.z);
+  w.hk = blockIdx.x / p.P;
+  w.chunk = blockIdx.x % p.P;
+  w.R = BM / p.G * p.G;
+  w.pairs = w.q.n * p.G;
+  w.c0 = (gridDim.y - 1 - blockIdx.y) * TILES;  // later rows see more keys: they start first
+  if (w.c0 * w.R >= w.pairs) return false;
+  tile_positions(p, w.q, w.c0 / TILES, TILES * w.R, w.pos_lo, w.pos_hi);
+  w.span = KeySpan(p, w.q, w.pos_lo, w.pos_hi, BN);
+  const int tiles = w.span.count(), per = p.chunk / BN;
+  w.chunks = chunks_of(p, tiles, BN);
+  if (w.chunk >= w.chunks) return false;
+  w.v0 = w.chunk * per;
+  const int v1 = w.chunk + 1 == w.chunks ? tiles : min(tiles, w.v0 + per);
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    int lo, hi, n = 0;
+    if ((w.c0 + t) * w.R < w.pairs) {
+      // Span tiles whose first key the tile's last row reaches, a prefix.
+      tile_positions(p, w.q, w.c0 + t, w.R, lo, hi);
+      const int last = min(hi, w.q.ctx - 1);
+      const int reach = last < 0 ? 0 : last / BN + 1;  // key tiles from 0 on
+      n = min(w.span.s_tiles, reach) + max(0, min(w.span.hi, reach) - w.span.lo);
+    }
+    w.nkv_t[t] = max(0, min(n, v1) - w.v0);
+  }
+  w.nkv = max(w.nkv_t[0], w.nkv_t[1]);
+  return true;
+}
+
+template <int D, int FMT, bool FP8>
+__global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
+paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                   const __grid_constant__ CUtensorMap tv, const Params p, const int box_log2) {
+  using L = Smem<D>;
+  using T = typename std::conditional<FMT == 1, __nv_bfloat16, __half>::type;
+  constexpr int KC = L::KC;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  uint64_t* q_full = bars;                // [TILES]
+  uint64_t* k_full = q_full + TILES;      // [NS]
+  uint64_t* v_full = k_full + NS;         // [NS]
+  uint64_t* kv_empty = v_full + NS;       // [NS]
+  uint64_t* s_full = kv_empty + NS;       // [TILES]
+  uint64_t* p_full = s_full + TILES;      // [TILES][2]
+  uint64_t* pv_done = p_full + 2 * TILES; // [TILES]
+  uint64_t* edge = pv_done + TILES;       // V boxes of a tile that is zeroed in places
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::TMEM_SLOT_OFF);
+  volatile uint32_t* pages = reinterpret_cast<volatile uint32_t*>(smem + L::PAGES_OFF);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  allow_dependents();
+  wait_prerequisites();
+  Item w;
+  if (!make_item(p, w)) return;  // the whole CTA alike
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < TILES; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[2 * t], BM);
+      mbar_init(&p_full[2 * t + 1], BM);
+      mbar_init(&pv_done[t], 1);
+    }
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&k_full[s], FP8 ? 4 : 1);
+      mbar_init(&v_full[s], FP8 ? 4 : 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    mbar_init(edge, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  uint8_t* sQ = smem + L::Q_OFF;
+  uint8_t* sK = smem + L::K_OFF;
+  uint8_t* sV = smem + L::V_OFF;
+  const int32_t* bt = p.block_tables + (int64_t)blockIdx.z * p.max_blocks;
+  // First key of the item's j-th tile.
+  auto key0_of = [&](int j) { return w.span.tile(w.v0 + j) * BN; };
+  // Whether some key of [a, a + n) is seen by a row of the item.
+  auto any_seen = [&](int a, int n) {
+    return a <= w.pos_hi && a < w.q.ctx &&
+           (p.window == 0 || w.pos_lo - (a + n - 1) < p.window || a < p.sinks);
+  };
+  auto all_seen_by_some = [&](int a, int n) {  // no key of [a, a + n) is unseen by every row
+    const int b = a + n - 1;
+    return b <= w.pos_hi && b < w.q.ctx && (p.window == 0 || w.pos_lo - a < p.window || b < p.sinks);
+  };
+
+  // Register split, 384 threads x 168 at launch: 128 x 96 + 256 x 200 = 63,488
+  // of 64,512. e4m3: 512 x 128 at launch: 128 x (56 + 88) + 256 x 184 = 65,536.
+  if (warp == 0) {
+    // ------------------------------------------------------------- loads --
+    reg_dealloc<FP8 ? 56 : 96>();
+    if (lane == 0) {
+      prefetch_tmap(&tq);
+      const int tokens = w.R / p.G;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) {
+        if (w.nkv_t[t] == 0) continue;
+        mbar_arrive_expect_tx(&q_full[t], KC * w.R * 128);
+        for (int kc = 0; kc < KC; ++kc)
+          tma_load_4d(sQ + (t * KC + kc) * CHUNK_BYTES, &tq, &q_full[t], kc * 64, 0, w.hk,
+                      w.q.row0 + (w.c0 + t) * tokens);
+      }
+    }
+    if constexpr (!FP8) {
+      const int box = 1 << box_log2;          // rows per TMA box: a page, 128 of a larger one
+      const int per_tile = BN >> box_log2;    // boxes per tile (at most 16)
+      bool ok = true;
+      int edges = 0;
+      // One lane per box: its page for the next tile is read a tile ahead.
+      auto page_of = [&](int j) -> int {
+        if (lane >= per_tile || j >= w.nkv) return -1;
+        const int key = key0_of(j) + lane * box;
+        if (!any_seen(key, box)) return -1;
+        const int id = bt[key >> p.bs_log2];
+        return id >= 0 && id < p.num_blocks ? id : -1;
+      };
+      int id = page_of(0);
+      for (int j = 0; ok && j < w.nkv; ++j) {
+        const int s = j % NS;
+        const int next = page_of(j + 1);
+        if (j >= NS && !mbar_wait_warp(&kv_empty[s], ((j / NS) - 1) & 1, 0x501)) break;
+        const int key0 = key0_of(j), row = (key0 + lane * box) & ((1 << p.bs_log2) - 1);
+        const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);  // bit per box
+        const bool clean = all_seen_by_some(key0, BN);
+        if (lane == 0) {
+          uint32_t m = 0;  // bit per 8 keys
+          for (int b = 0; b < per_tile; ++b)
+            if ((have >> b) & 1) m |= ((1u << (box / 8)) - 1u) << (b * (box / 8));
+          pages[s] = m;
+          mbar_arrive_expect_tx(&k_full[s], KC * CHUNK_BYTES);
+          mbar_arrive_expect_tx(clean ? &v_full[s] : edge, KC * CHUNK_BYTES);
+        }
+        __syncwarp();
+        // A block past the cache reads as zeros.
+        const int blk = id >= 0 ? id : p.num_blocks;
+        if (lane < per_tile)
+          for (int kc = 0; kc < KC; ++kc)
+            tma_load_4d(sK + (s * KC + kc) * CHUNK_BYTES + lane * box * 128, &tk, &k_full[s], kc * 64,
+                        row, w.hk, blk);
+        __syncwarp();
+        if (lane < per_tile)
+          for (int kc = 0; kc < KC; ++kc)
+            tma_load_4d(sV + (s * KC + kc) * CHUNK_BYTES + lane * box * 128, &tv,
+                        clean ? &v_full[s] : edge, kc * 64, row, w.hk, blk);
+        if (!clean) {
+          if (!mbar_wait_warp(edge, edges & 1, 0x502)) break;
+          ++edges;
+          for (int r = lane; r < BN; r += 32)
+            if (!seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key0 + r))
+              for (int kc = 0; kc < KC; ++kc)
+                for (int c = 0; c < 8; ++c)
+                  *reinterpret_cast<uint4*>(sV + (s * KC + kc) * CHUNK_BYTES + r * 128 + c * 16) =
+                      make_uint4(0u, 0u, 0u, 0u);
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[s]);
+        }
+        id = next;
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------- MMA issue --
+    reg_dealloc<FP8 ? 56 : 96>();
+    if (lane == 0) {
+      constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, FMT, 0, 0);
+      constexpr uint32_t IDESC_PV = idesc_f16(BM, D, FMT, 0, 1);
+      const uint32_t q_base = smem_u32(sQ), k_base = smem_u32(sK), v_base = smem_u32(sV);
+      auto issue_qk = [&](int t, int j) {
+        const int s = j % NS;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk / 4) * CHUNK_BYTES + (kk % 4) * 32;
+          mma_ss(tmem + t * 128, smem_desc_sw128(q_base + t * KC * CHUNK_BYTES + off, 16, 1024),
+                 smem_desc_sw128(k_base + s * KC * CHUNK_BYTES + off, 16, 1024), IDESC_QK, kk > 0);
+        }
+        mma_commit(&s_full[t]);
+      };
+      // PV over keys [64 h, 64 h + 64) of the tile; the second half commits pv_done.
+      auto issue_pv_half = [&](int t, int j, int h) {
+        const int s = j % NS;
+#pragma unroll
+        for (int k4 = 0; k4 < BN / 32; ++k4) {
+          const int kk = h * (BN / 32) + k4;
+          mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
+                 smem_desc_sw128(v_base + s * KC * CHUNK_BYTES + kk * 2048, CHUNK_BYTES, 1024),
+                 IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+        }
+        if (h == 1) mma_commit(&pv_done[t]);
+      };
+      bool ok = true;
+      for (int t = 0; t < TILES && ok; ++t)
+        if (w.nkv_t[t] > 0 && !mbar_wait(&q_full[t], 0, 0x511)) ok = false;
+      if (ok && w.nkv > 0 && !mbar_wait(&k_full[0], 0, 0x512)) ok = false;
+      tc_fence_after();
+      for (int t = 0; ok && t < TILES; ++t)
+        if (w.nkv_t[t] > 0) issue_qk(t, 0);
+      for (int j = 0; ok && j < w.nkv; ++j) {
+        const int s = j % NS;
+        if (!mbar_wait(&v_full[s], (j / NS) & 1, 0x513)) { ok = false; break; }
+        for (int t = 0; t < TILES; ++t) {
+          if (j >= w.nkv_t[t]) continue;
+          if (!mbar_wait(&p_full[2 * t], j & 1, 0x514)) { ok = false; break; }
+          tc_fence_after();
+          issue_pv_half(t, j, 0);
+          if (!mbar_wait(&p_full[2 * t + 1], j & 1, 0x515)) { ok = false; break; }
+          tc_fence_after();
+          issue_pv_half(t, j, 1);
+          if (j + 1 < w.nkv_t[t]) {
+            if (!mbar_wait(&k_full[(j + 1) % NS], ((j + 1) / NS) & 1, 0x516)) { ok = false; break; }
+            tc_fence_after();
+            issue_qk(t, j + 1);
+          }
+        }
+        if (ok) mma_commit(&kv_empty[s]);
+      }
+    }
+  } else if (warp < 4) {
+    reg_dealloc<FP8 ? 56 : 96>();  // idle members of the first warpgroup
+  } else if (warp < 12) {
+    // ----------------------------------------------------------- softmax --
+    reg_alloc<FP8 ? 184 : 200>();
+    const int t = (warp >> 2) - 1;
+    const int row = threadIdx.x - 128 * (t + 1);  // TMEM lane
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float sl2 = p.scale_log2;
+    const int nkv_t = t == 0 ? w.nkv_t[0] : w.nkv_t[1];
+    const int pr = (w.c0 + t) * w.R + row;
+    const bool mine = row < w.R && pr < w.pairs;
+    const int pos = w.q.pos0 + pr / p.G;
+    int tile_lo = 0, tile_hi = 0;
+    if ((w.c0 + t) * w.R < w.pairs) tile_positions(p, w.q, w.c0 + t, w.R, tile_lo, tile_hi);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < nkv_t; ++j) {
+      const int s = j % NS;
+      // (k_full has long completed: its wait orders the reads of `pages`.)
+      if (!mbar_wait_warp(&s_full[t], j & 1, 0x521) ||
+          !mbar_wait_warp(&k_full[s], (j / NS) & 1, 0x522)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t sr[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld32(lane_addr + t * 128 + 32 * i, sr[i]);
+      const uint32_t have = pages[s];
+      const int kv0 = key0_of(j);
+      tmem_ld_wait();
+      const int last = kv0 + BN - 1;
+      const bool whole = last <= tile_lo && last < w.q.ctx && have == 0xffffu &&
+                         (p.window == 0 || tile_hi - kv0 < p.window || last < p.sinks);
+      if (!whole) {
+        const int hi = min(w.q.ctx, pos + 1) - kv0;                  // columns from hi on are hidden
+        const int lo = p.window > 0 ? pos - p.window + 1 - kv0 : 0;  // below lo: sinks only
+        const int sk = p.window > 0 ? p.sinks - kv0 : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int cc = 0; cc < 32; ++cc) {
+            const int c = 32 * i + cc;
+            if (c >= hi || (c < lo && c >= sk) || !((have >> (c >> 3)) & 1))
+              sr[i][cc] = __float_as_uint(-INFINITY);
+          }
+      }
+      const float mx = row_max(sr);
+      const float m_new = fmaxf(m, mx * sl2);
+      float alpha = 1.f;
+      const bool rescale = m_new > m + RESCALE_THRESHOLD;
+      if (rescale) {
+        alpha = ex2(m - m_new);
+        m = m_new;
+        l *= alpha;
+      }
+      const float m_use = (m == -INFINITY) ? 0.f : m;
+      float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
+                      make_float2(0.f, 0.f)};
+      const float2 sl2_2 = make_float2(sl2, sl2), negm2 = make_float2(-m_use, -m_use);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 2 * h; i < 2 * h + 2; ++i) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int cc = 0; cc < 16; ++cc) {
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[i][2 * cc]),
+                                                    __uint_as_float(sr[i][2 * cc + 1])),
+                                        sl2_2, negm2);
+            const float2 pp = make_float2(ex2(x.x), ex2(x.y));
+            l2[cc & 3] = __fadd2_rn(l2[cc & 3], pp);
+            pk[cc] = FMT == 1 ? pack_bf16(pp.x, pp.y) : pack_f16(pp.x, pp.y);
+          }
+#pragma unroll
+          for (int cc = 0; cc < 16; ++cc) sr[h][(i & 1) * 16 + cc] = pk[cc];
+        }
+        tmem_st32(lane_addr + t * 128 + 32 * h, sr[h]);
+        // O is rescaled before the first half's PV accumulates into it; PV_t(j-1)
+        // has completed: s_full(j) follows it in issue order.
+        if (h == 0 && __any_sync(0xffffffffu, rescale && j > 0)) {
+          const float a = (rescale && j > 0) ? alpha : 1.f;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t ov[32];
+            tmem_ld32(lane_addr + 256 + t * 128 + 32 * i, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int cc = 0; cc < 32; ++cc) ov[cc] = __float_as_uint(__uint_as_float(ov[cc]) * a);
+            tmem_st32(lane_addr + 256 + t * 128 + 32 * i, ov);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[2 * t + h]);
+      }
+      const float2 a2 = __fadd2_rn(__fadd2_rn(l2[0], l2[1]), __fadd2_rn(l2[2], l2[3]));
+      l += a2.x + a2.y;
+    }
+    if (ok && nkv_t > 0) {
+      if (!mbar_wait_warp(&pv_done[t], (nkv_t - 1) & 1, 0x523)) ok = false;
+      tc_fence_after();
+    }
+    if (ok) {
+      const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;  // NaN sums give NaN
+      const bool none = l == 0.f;  // a row without keys: 0, whatever V holds
+      const int tok = w.q.row0 + pr / p.G, h = w.hk * p.G + pr % p.G;
+      const int64_t at = ((int64_t)tok * p.Hq + h) * p.P + w.chunk;
+      uint8_t* orow = static_cast<uint8_t*>(p.o) +
+                      2 * ((int64_t)tok * p.so_t + (int64_t)h * p.so_h);
+      const bool st32 = (reinterpret_cast<uintptr_t>(orow) & 31) == 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        uint32_t ov[32];
+        if (nkv_t > 0) {
+          tmem_ld32(lane_addr + 256 + t * 128 + 32 * i, ov);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int cc = 0; cc < 32; ++cc)
+          ov[cc] = none ? 0u : __float_as_uint(__uint_as_float(ov[cc]) * inv);
+        if (mine && w.chunks > 1) {
+#pragma unroll
+          for (int v8 = 0; v8 < 4; ++v8) st_global_v8(p.part_o + at * D + 32 * i + 8 * v8, &ov[8 * v8]);
+        } else if (mine) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int cc = 0; cc < 16; ++cc) {
+            const float a0 = __uint_as_float(ov[2 * cc]), a1 = __uint_as_float(ov[2 * cc + 1]);
+            pk[cc] = FMT == 1 ? pack_bf16(a0, a1) : pack_f16(a0, a1);
+          }
+          if (st32) {
+#pragma unroll
+            for (int v8 = 0; v8 < 2; ++v8) st_global_v8(orow + 64 * i + 32 * v8, &pk[8 * v8]);
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(orow + 64 * i);
+#pragma unroll
+            for (int v4 = 0; v4 < 4; ++v4)
+              dst[v4] = make_uint4(pk[4 * v4], pk[4 * v4 + 1], pk[4 * v4 + 2], pk[4 * v4 + 3]);
+          }
+        }
+        __syncwarp();
+      }
+      if (mine) {
+        const float lse2 = none ? -INFINITY : m + log2f(l);
+        if (w.chunks > 1)
+          p.part_lse[at] = lse2;
+        else if (p.lse != nullptr)
+          p.lse[(int64_t)h * p.T + tok] = lse2 * 0.69314718055994531f;
+      }
+      tc_fence_before();
+    }
+  } else {
+    // ----------------------------------------------------------- convert --
+    reg_dealloc<88>();
+    if constexpr (FP8) {
+      constexpr int CPR = D / 16;           // 16-byte pieces of a cached row
+      constexpr int RPP = 128 / CPR;        // rows per pass of the 128 threads
+      constexpr int PASSES = BN / RPP;
+      const int tid = threadIdx.x - 384, c = tid % CPR, r0 = tid / CPR;
+      const int bs = 1 << p.bs_log2;
+      // Registers of one tile: 16 bytes and a scale of rows r0, r0 + RPP, ...;
+      // rows that no row of the item sees, or whose page is missing, are zeros.
+      struct Tile {
+        uint4 x[PASSES];
+        uint32_t e[PASSES];
+      };
+      auto load = [&](Tile& r, const uint8_t* cache, const uint8_t* scale, int j) {
+        const int key0 = key0_of(j);
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const int key = key0 + r0 + i * RPP;
+          r.x[i] = make_uint4(0u, 0u, 0u, 0u);
+          r.e[i] = 127;
+          if (seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key)) {
+            const int id = bt[key >> p.bs_log2];
+            if (id >= 0 && id < p.num_blocks) {
+              const int64_t cell = ((int64_t)id * p.Hkv + w.hk) * bs + (key & (bs - 1));
+              r.x[i] = __ldg(reinterpret_cast<const uint4*>(cache + cell * D) + c);
+              r.e[i] = scale[cell];
+            }
+          }
+        }
+      };
+      auto store = [&](const Tile& r, uint8_t* tile) {
+        const int kc = c / 4;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          const int row = r0 + i * RPP;
+          const float f = e8m0_to_float((int)r.e[i]);
+          const uint32_t words[4] = {r.x[i].x, r.x[i].y, r.x[i].z, r.x[i].w};
+          uint32_t o[8];
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            float y[4];
+            e4m3x4_to_float(words[q4], y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = clamp_finite<T>(y[e] * f);
+            o[2 * q4] = FMT == 1 ? pack_bf16(y[0], y[1]) : pack_f16(y[0], y[1]);
+            o[2 * q4 + 1] = FMT == 1 ? pack_bf16(y[2], y[3]) : pack_f16(y[2], y[3]);
+          }
+          uint8_t* base = tile + kc * CHUNK_BYTES + row * 128;
+          // Halves in alternating order, so that 8 lanes of a row touch every bank once.
+          const int first = (c >> 2) & 1, piece = (c & 3) * 2;
+          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(base + (((piece + first) ^ (row & 7)) << 4)) = first ? hi : lo;
+          *reinterpret_cast<uint4*>(base + (((piece + 1 - first) ^ (row & 7)) << 4)) = first ? lo : hi;
+        }
+      };
+      bool ok = true;
+      auto page_at = [&](int j) -> bool {  // lane b < 16: the page of keys [8 b, 8 b + 8)
+        if (lane >= BN / 8 || j >= w.nkv) return false;
+        const int key = key0_of(j) + 8 * lane;
+        if (key >= w.q.ctx) return false;
+        const int id = bt[key >> p.bs_log2];
+        return id >= 0 && id < p.num_blocks;
+      };
+      Tile kt, vt;
+      bool there = page_at(0);
+      if (w.nkv > 0) load(kt, static_cast<const uint8_t*>(p.k_cache), p.k_scale, 0);
+      for (int j = 0; ok && j < w.nkv; ++j) {
+        const int s = j % NS;
+        load(vt, static_cast<const uint8_t*>(p.v_cache), p.v_scale, j);
+        if (j >= NS && !mbar_wait_warp(&kv_empty[s], ((j / NS) - 1) & 1, 0x531)) break;
+        if (warp == 12) {
+          // Pages by 8 keys, for the softmax warps (ordered by this warp's arrival).
+          const uint32_t mask = __ballot_sync(0xffffffffu, there);
+          if (lane == 0) pages[s] = mask;
+          there = page_at(j + 1);
+        }
+        store(kt, sK + s * KC * CHUNK_BYTES);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_full[s]);
+        if (j + 1 < w.nkv) load(kt, static_cast<const uint8_t*>(p.k_cache), p.k_scale, j + 1);
+        store(vt, sV + s * KC * CHUNK_BYTES);
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[s]);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// q as [T, Hkv, G, D]: boxes of 64 columns, G heads, the tokens of one tile.
+static int make_q_map(CUtensorMap* map, const Params& p, int dtype) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled unavailable (no CUDA driver?)");
+    return LSB_ERR_CUDA;
+  }
+  cuuint64_t dims[4] = {(cuuint64_t)p.D, (cuuint64_t)p.G, (cuuint64_t)p.Hkv, (cuuint64_t)p.T};
+  // A dim of one has no stride of its own: any multiple of 16 bytes will do.
+  const int64_t sg = p.Hq > 1 ? p.sq_h : p.D, st = p.T > 1 ? p.sq_t : p.D;
+  cuuint64_t strides[3] = {(cuuint64_t)(sg * 2), (cuuint64_t)(sg * p.G * 2), (cuuint64_t)(st * 2)};
+  cuuint32_t box[4] = {64, (cuuint32_t)p.G, 1, (cuuint32_t)(BM / p.G)};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, dtype == LSB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                   4, const_cast<void*>(p.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LSB_ERR_CUDA;
+  }
+  return LSB_OK;
+}
+
+template <int D, int FMT, bool FP8>
+static int launch(const Params& p, int dtype, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  int rc = make_q_map(&mq, p, dtype);
+  const int box_log2 = std::min(p.bs_log2, 7);
+  const int64_t bs = 1LL << p.bs_log2;
+  const int64_t sc[4] = {(int64_t)p.Hkv * bs * D, bs * D, D, 1};  // [num_blocks, Hkv, bs, D]
+  if (!FP8) {
+    if (!rc) rc = make_bhnd_map(&mk, p.k_cache, dtype, p.num_blocks, p.Hkv, bs, D, sc, 64, 1u << box_log2);
+    if (!rc) rc = make_bhnd_map(&mv, p.v_cache, dtype, p.num_blocks, p.Hkv, bs, D, sc, 64, 1u << box_log2);
+  } else {
+    mk = mv = mq;  // not used
+  }
+  if (rc) return rc;
+  auto kern = paged_chunk_kernel<D, FMT, FP8>;
+  static SmemLimit limit;
+  if (int rc_ = limit.ensure(kern, Smem<D>::ALLOC, "paged_attn smem attribute")) return rc_;
+  const int64_t R = (int64_t)(BM / p.G * p.G) * TILES;
+  const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)(((int64_t)p.max_q * p.G + R - 1) / R), (unsigned)p.S);
+  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(FP8 ? 512 : 384), Smem<D>::ALLOC, st, mq, mk, mv, p, box_log2),
+              "paged_attn");
+  return LSB_OK;
+}
+
+}  // namespace tc
+
+bool tc_eligible(const Params& p, int dtype, bool kv_fp8) {
+  if (dtype != LSB_DTYPE_BF16 && dtype != LSB_DTYPE_F16) return false;
+  if ((p.D != 64 && p.D != 128) || p.bs_log2 < 3 || p.G > tc::BM) return false;
+  if (!(p.scale_log2 > 0.f)) return false;  // the running maximum is taken before the scale
+  // TMA: 16-byte aligned bases and strides; rows of o are written 16 bytes at a time.
+  if (!aligned16(p.q) || p.sq_t % 8 != 0 || p.sq_h % 8 != 0 || p.sq_t < 0 || p.sq_h < 0) return false;
+  if (!aligned16(p.o) || p.so_t % 8 != 0 || p.so_h % 8 != 0) return false;
+  if (!aligned16(p.k_cache) || !aligned16(p.v_cache)) return false;
+  if (p.T > 1 && p.sq_t == 0) return false;
+  if (p.Hq > 1 && p.sq_h == 0) return false;
+  const int64_t R = (int64_t)(tc::BM / p.G * p.G) * tc::TILES;
+  return ((int64_t)p.max_q * p.G + R - 1) / R <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff;
+}
+
+int launch_tc(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
+  const bool bf = dtype == LSB_DTYPE_BF16;
+  if (p.D == 128) {
+    if (kv_fp8) return bf ? tc::launch<128, 1, true>(p, dtype, st) : tc::launch<128, 0, true>(p, dtype, st);
+    return bf ? tc::launch<128, 1, false>(p, dtype, st) : tc::launch<128, 0, false>(p, dtype, st);
+  }
+  if (kv_fp8) return bf ? tc::launch<64, 1, true>(p, dtype, st) : tc::launch<64, 0, true>(p, dtype, st);
+  return bf ? tc::launch<64, 1, false>(p, dtype, st) : tc::launch<64, 0, false>(p, dtype, st);
+}
+
+}  // namespace pa
+
+int paged_attn_tc_device_error(bool reset) { return sm100::tu_device_error(reset); }
+
+}  // namespace lsb

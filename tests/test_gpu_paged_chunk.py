@@ -44,12 +44,12 @@ def _check(b, window=None, sinks=0, impl=_lib.IMPL_AUTO, **kw):
     return out, lse
 
 
-IMPLS = {"auto": _lib.IMPL_AUTO, "simt": _lib.IMPL_SIMT, "rows": _lib.IMPL_ROWS}
+IMPLS = {"auto": _lib.IMPL_AUTO, "simt": _lib.IMPL_SIMT, "rows": _lib.IMPL_ROWS, "tc": _lib.IMPL_TCGEN05}
 
 
 def _skip_if_not_served(impl, dtype):
-    if impl == "rows" and dtype == F32:
-        pytest.skip("the few-rows kernel serves 16-bit types")
+    if impl in ("rows", "tc") and dtype == F32:
+        pytest.skip("the tensor-core kernels serve 16-bit types")
 LENS = [  # cached tokens, new tokens
     ([1], [1]),
     ([40, 17, 1, 0, 16], [3, 17, 1, 0, 16]),            # whole prompts, an empty sequence
