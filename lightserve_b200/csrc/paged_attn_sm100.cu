@@ -79,6 +79,11 @@ __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// The n lowest bits set (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u;
+}
+
 __device__ __forceinline__ float row_max(const uint32_t (&sr)[4][32]) {
   float mx8[8];
 #pragma unroll
@@ -367,17 +372,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       const bool whole = last <= tile_lo && last < w.q.ctx && have == 0xffffu &&
                          (p.window == 0 || tile_hi - kv0 < p.window || last < p.sinks);
       if (!whole) {
-        const int hi = min(w.q.ctx, pos + 1) - kv0;                  // columns from hi on are hidden
-        const int lo = p.window > 0 ? pos - p.window + 1 - kv0 : 0;  // below lo: sinks only
+        // Visible columns as bits, 32 columns a word: below hi, from lo on (or a
+        // sink, below sk), and in a page that is there.
+        const int hi = min(w.q.ctx, pos + 1) - kv0;
+        const int lo = p.window > 0 ? pos - p.window + 1 - kv0 : 0;
         const int sk = p.window > 0 ? p.sinks - kv0 : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+          uint32_t pg = 0;
 #pragma unroll
-          for (int cc = 0; cc < 32; ++cc) {
-            const int c = 32 * i + cc;
-            if (c >= hi || (c < lo && c >= sk) || !((have >> (c >> 3)) & 1))
-              sr[i][cc] = __float_as_uint(-INFINITY);
-          }
+          for (int b = 0; b < 4; ++b) pg |= (0u - ((have >> (4 * i + b)) & 1u)) & (0xffu << (8 * b));
+          const uint32_t bits =
+              low_bits(hi - 32 * i) & (~low_bits(lo - 32 * i) | low_bits(sk - 32 * i)) & pg;
+#pragma unroll
+          for (int cc = 0; cc < 32; ++cc)
+            if (!((bits >> cc) & 1)) sr[i][cc] = __float_as_uint(-INFINITY);
+        }
       }
       const float mx = row_max(sr);
       const float m_new = fmaxf(m, mx * sl2);
@@ -493,26 +503,35 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       constexpr int PASSES = BN / RPP;
       const int tid = threadIdx.x - 384, c = tid % CPR, r0 = tid / CPR;
       const int bs = 1 << p.bs_log2;
+      // Page ids of a tile, lane b < 16 holding that of keys [8 b, 8 b + 8) (-1:
+      // none), fetched a tile ahead of the rows they lead to.
+      auto fetch_ids = [&](int j) -> int {
+        if (lane >= BN / 8 || j >= w.nkv) return -1;
+        const int key = key0_of(j) + 8 * lane;
+        if (key >= w.q.ctx) return -1;
+        const int id = bt[key >> p.bs_log2];
+        return id >= 0 && id < p.num_blocks ? id : -1;
+      };
       // Registers of one tile: 16 bytes and a scale of rows r0, r0 + RPP, ...;
       // rows that no row of the item sees, or whose page is missing, are zeros.
       struct Tile {
         uint4 x[PASSES];
         uint32_t e[PASSES];
       };
-      auto load = [&](Tile& r, const uint8_t* cache, const uint8_t* scale, int j) {
+      auto load = [&](Tile& r, const uint8_t* cache, const uint8_t* scale, int j, int ids) {
         const int key0 = key0_of(j);
+        const bool clean = all_seen_by_some(key0, BN);
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
-          const int key = key0 + r0 + i * RPP;
+          const int row = r0 + i * RPP, key = key0 + row;
+          const int id = __shfl_sync(0xffffffffu, ids, row >> 3);
+          const bool ok = id >= 0 && (clean || seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key));
+          const int64_t cell = ((int64_t)max(id, 0) * p.Hkv + w.hk) * bs + (key & (bs - 1));
           r.x[i] = make_uint4(0u, 0u, 0u, 0u);
           r.e[i] = 127;
-          if (seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key)) {
-            const int id = bt[key >> p.bs_log2];
-            if (id >= 0 && id < p.num_blocks) {
-              const int64_t cell = ((int64_t)id * p.Hkv + w.hk) * bs + (key & (bs - 1));
-              r.x[i] = __ldg(reinterpret_cast<const uint4*>(cache + cell * D) + c);
-              r.e[i] = scale[cell];
-            }
+          if (ok) {
+            r.x[i] = __ldg(reinterpret_cast<const uint4*>(cache + cell * D) + c);
+            r.e[i] = __ldg(scale + cell);
           }
         }
       };
@@ -526,12 +545,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           uint32_t o[8];
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
-            float y[4];
-            e4m3x4_to_float(words[q4], y);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = clamp_finite<T>(y[e] * f);
-            o[2 * q4] = FMT == 1 ? pack_bf16(y[0], y[1]) : pack_f16(y[0], y[1]);
-            o[2 * q4 + 1] = FMT == 1 ? pack_bf16(y[2], y[3]) : pack_f16(y[2], y[3]);
+            for (int e = 0; e < 2; ++e) {
+              const float2 y = __fmul2_rn(
+                  f16x2_to_float2(cvt_e4m3x2_f16x2((uint16_t)(words[q4] >> (16 * e)))), make_float2(f, f));
+              if constexpr (FMT == 1) {
+                o[2 * q4 + e] = pack_bf16(y.x, y.y);
+              } else {  // a value lifted past fp16's range stays at its largest
+                const __half2 top = __float2half2_rn(65504.f);
+                const uint32_t z = pack_f16(y.x, y.y);
+                const __half2 c2 = __hmax2_nan(
+                    __hmin2_nan(*reinterpret_cast<const __half2*>(&z), top), __hneg2(top));
+                o[2 * q4 + e] = *reinterpret_cast<const uint32_t*>(&c2);
+              }
+            }
           }
           uint8_t* base = tile + kc * CHUNK_BYTES + row * 128;
           // Halves in alternating order, so that 8 lanes of a row touch every bank once.
@@ -542,31 +569,25 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         }
       };
       bool ok = true;
-      auto page_at = [&](int j) -> bool {  // lane b < 16: the page of keys [8 b, 8 b + 8)
-        if (lane >= BN / 8 || j >= w.nkv) return false;
-        const int key = key0_of(j) + 8 * lane;
-        if (key >= w.q.ctx) return false;
-        const int id = bt[key >> p.bs_log2];
-        return id >= 0 && id < p.num_blocks;
-      };
+      const uint8_t* kc = static_cast<const uint8_t*>(p.k_cache);
+      const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
       Tile kt, vt;
-      bool there = page_at(0);
-      if (w.nkv > 0) load(kt, static_cast<const uint8_t*>(p.k_cache), p.k_scale, 0);
-      for (int j = 0; ok && j < w.nkv; ++j) {
+      int ids = fetch_ids(0), next = fetch_ids(1);
+      if (w.nkv > 0) load(kt, kc, p.k_scale, 0, ids);
+      for (int j = 0; j < w.nkv; ++j) {
         const int s = j % NS;
-        load(vt, static_cast<const uint8_t*>(p.v_cache), p.v_scale, j);
+        load(vt, vc, p.v_scale, j, ids);
         if (j >= NS && !mbar_wait_warp(&kv_empty[s], ((j / NS) - 1) & 1, 0x531)) break;
-        if (warp == 12) {
-          // Pages by 8 keys, for the softmax warps (ordered by this warp's arrival).
-          const uint32_t mask = __ballot_sync(0xffffffffu, there);
-          if (lane == 0) pages[s] = mask;
-          there = page_at(j + 1);
-        }
+        // Pages by 8 keys, for the softmax warps (ordered by this warp's arrival).
+        const uint32_t have = __ballot_sync(0xffffffffu, ids >= 0);
+        if (tid == 0) pages[s] = have;
+        ids = next;
+        next = fetch_ids(j + 2);
         store(kt, sK + s * KC * CHUNK_BYTES);
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&k_full[s]);
-        if (j + 1 < w.nkv) load(kt, static_cast<const uint8_t*>(p.k_cache), p.k_scale, j + 1);
+        if (j + 1 < w.nkv) load(kt, kc, p.k_scale, j + 1, ids);
         store(vt, sV + s * KC * CHUNK_BYTES);
         fence_async_shared();
         __syncwarp();
