@@ -8,15 +8,15 @@
 // conditional rescale, P packed to 16 bits over S in two halves, O_t += P_t V
 // (TS), the two query tiles' MMA batches and softmaxes alternating. What
 // differs is where K and V come from and which keys count:
-//  * 16-bit cache: one TMA box per page, head and 64-column half. A page's rows
-//    land where the 128-byte swizzle wants them, since boxes start at multiples
-//    of 8 rows, so a tile of pages looks like a tile of one tensor. Pages that do
-//    not exist, or that no row sees, are fetched at an out-of-range block: zeros.
-//  * e4m3 cache: a converter warpgroup reads the rows (16 bytes a thread, one
-//    tile ahead in registers), multiplies by the row's power of two in fp32 and
-//    rounds to q's type, which is exact in bf16 (and in fp16 within its range),
-//    and writes the swizzled tile. Converting in the MMA's shadow costs no time
-//    on the S -> softmax -> P chain that bounds the kernel.
+//  * 16-bit cache: one TMA box per page and head (the cache is a tensor of
+//    8-row groups, so the box's atoms land as the MMA's descriptors want them; a
+//    box per 64-column half took 13% longer over pages of 16). Pages that do not
+//    exist, or that no row sees, are fetched past the end: zeros.
+//  * e4m3 cache: two converter warpgroups, for K and V, read the rows (16 bytes a
+//    thread, one tile ahead in registers), multiply by the row's power of two in
+//    fp32 and round to q's type, which is exact in bf16 (and in fp16 within its
+//    range), and write the swizzled tiles, in the shadow of the S -> softmax -> P
+//    chain that bounds the kernel.
 //  * V rows that no row of the item sees (past the context, between sinks and
 //    window) are zeroed in shared memory, so that what such cells hold never
 //    meets a weight of 0; the tiles that need it are the ends of a span.
@@ -24,7 +24,7 @@
 //    token r / G, head r % G.
 //
 // Warps: 0 loads (Q; K, V of a 16-bit cache), 1 issues MMAs and owns TMEM,
-// 4-7 and 8-11 softmax of query tile 0 and 1, 12-15 convert (e4m3 only).
+// 4-7 and 8-11 softmax of query tile 0 and 1; e4m3: 12-15 convert K, 16-19 V.
 // TMEM: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512) columns. Every
 // mbarrier wait is bounded; on a timeout the error word is set, the role ends,
 // TMEM is freed and the CTA exits.
@@ -45,21 +45,26 @@ constexpr int BM = 128;
 constexpr int BN = TC_TK;
 constexpr int TILES = 2;
 constexpr int NS = 2;  // K/V ring stages
-constexpr int CHUNK_BYTES = 128 * 128;  // [128 rows][64 columns] of 16 bits
+constexpr int CHUNK_BYTES = 128 * 128;  // Q: [128 rows][64 columns] of 16 bits
+// K and V tiles are rows of 128-byte-swizzled atoms (8 keys x 64 columns, 1024
+// bytes): [key / 8][column / 64][8 keys][64 columns], the order in which one
+// TMA box over [cache rows / 8, D / 64, 8, 64] delivers a whole page.
+constexpr int ATOM = 1024;
 constexpr float RESCALE_THRESHOLD = 8.0f;
 
 template <int D>
 struct Smem {
   static constexpr int KC = D / 64;
+  static constexpr int TILE = KC * CHUNK_BYTES;  // bytes of a K or V tile
   static constexpr int Q_OFF = 0;
   static constexpr int K_OFF = Q_OFF + TILES * KC * CHUNK_BYTES;
   static constexpr int V_OFF = K_OFF + NS * KC * CHUNK_BYTES;
   static constexpr int BAR_OFF = V_OFF + NS * KC * CHUNK_BYTES;
-  // q_full[2], k_full[NS], v_full[NS], kv_empty[NS], s_full[2], p_full[2][2], pv_done[2], edge
-  static constexpr int NBAR = TILES + 3 * NS + 4 * TILES + 1;
+  // q_full[2], k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full[2], p_full[2][2],
+  // pv_done[2], edge
+  static constexpr int NBAR = TILES + 4 * NS + 4 * TILES + 1;
   static constexpr int TMEM_SLOT_OFF = BAR_OFF + NBAR * 8;
-  static constexpr int PAGES_OFF = TMEM_SLOT_OFF + 16;  // [NS] bit per 8 keys: page there
-  static constexpr int BYTES = PAGES_OFF + NS * 4;
+  static constexpr int BYTES = TMEM_SLOT_OFF + 16;
   static constexpr int ALLOC = BYTES + 1024;  // slack for 1024-byte alignment
 };
 
@@ -84,12 +89,13 @@ __device__ __forceinline__ uint32_t low_bits(int n) {
   return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u;
 }
 
-__device__ __forceinline__ float row_max(const uint32_t (&sr)[4][32]) {
+template <int N>
+__device__ __forceinline__ float row_max(const uint32_t (&sr)[N][32]) {
   float mx8[8];
 #pragma unroll
   for (int u = 0; u < 8; ++u) mx8[u] = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int cc = 0; cc < 32; cc += 2)
       mx8[(cc >> 1) & 7] = max3f(mx8[(cc >> 1) & 7], __uint_as_float(sr[i][cc]),
@@ -143,7 +149,7 @@ __device__ __forceinline__ bool make_item(const Params& p, Item& w) {
 }
 
 template <int D, int FMT, bool FP8>
-__global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
+__global__ void __launch_bounds__(FP8 ? 640 : 384, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const Params p, const int box_log2) {
   using L = Smem<D>;
@@ -155,13 +161,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   uint64_t* q_full = bars;                // [TILES]
   uint64_t* k_full = q_full + TILES;      // [NS]
   uint64_t* v_full = k_full + NS;         // [NS]
-  uint64_t* kv_empty = v_full + NS;       // [NS]
-  uint64_t* s_full = kv_empty + NS;       // [TILES]
+  // K is free after its QK, V a step later after its PV: the next K's load or
+  // conversion has a whole step to hide behind.
+  uint64_t* k_empty = v_full + NS;        // [NS]
+  uint64_t* v_empty = k_empty + NS;       // [NS]
+  uint64_t* s_full = v_empty + NS;        // [TILES]
   uint64_t* p_full = s_full + TILES;      // [TILES][2]
   uint64_t* pv_done = p_full + 2 * TILES; // [TILES]
   uint64_t* edge = pv_done + TILES;       // V boxes of a tile that is zeroed in places
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::TMEM_SLOT_OFF);
-  volatile uint32_t* pages = reinterpret_cast<volatile uint32_t*>(smem + L::PAGES_OFF);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   allow_dependents();
@@ -180,7 +188,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     for (int s = 0; s < NS; ++s) {
       mbar_init(&k_full[s], FP8 ? 4 : 1);
       mbar_init(&v_full[s], FP8 ? 4 : 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_empty[s], 1);
     }
     mbar_init(edge, 1);
     fence_barrier_init();
@@ -209,11 +218,21 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     return b <= w.pos_hi && b < w.q.ctx && (p.window == 0 || w.pos_lo - a < p.window || b < p.sinks);
   };
 
+  // Page ids of the item's j-th tile, lane b < 16 holding that of keys
+  // [8 b, 8 b + 8); -1: no such page. Fetched a tile ahead of their use.
+  auto fetch_ids = [&](int j) -> int {
+    if (lane >= BN / 8 || j >= w.nkv) return -1;
+    const int key = key0_of(j) + 8 * lane;
+    if (key >= w.q.ctx) return -1;
+    const int id = bt[key >> p.bs_log2];
+    return id >= 0 && id < p.num_blocks ? id : -1;
+  };
+
   // Register split, 384 threads x 168 at launch: 128 x 96 + 256 x 200 = 63,488
-  // of 64,512. e4m3: 512 x 128 at launch: 128 x (56 + 88) + 256 x 184 = 65,536.
+  // of 64,512. e4m3: 640 x 96 at launch: 128 x 48 + 256 x 136 + 256 x 80 = 61,440.
   if (warp == 0) {
     // ------------------------------------------------------------- loads --
-    reg_dealloc<FP8 ? 56 : 96>();
+    reg_dealloc<FP8 ? 48 : 96>();
     if (lane == 0) {
       prefetch_tmap(&tq);
       const int tokens = w.R / p.G;
@@ -228,45 +247,30 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     }
     if constexpr (!FP8) {
       const int box = 1 << box_log2;          // rows per TMA box: a page, 128 of a larger one
-      const int per_tile = BN >> box_log2;    // boxes per tile (at most 16)
-      bool ok = true;
+      const int per_tile = BN >> box_log2;    // boxes per tile (at most 16): one lane each
       int edges = 0;
-      // One lane per box: its page for the next tile is read a tile ahead.
-      auto page_of = [&](int j) -> int {
-        if (lane >= per_tile || j >= w.nkv) return -1;
-        const int key = key0_of(j) + lane * box;
-        if (!any_seen(key, box)) return -1;
-        const int id = bt[key >> p.bs_log2];
-        return id >= 0 && id < p.num_blocks ? id : -1;
-      };
-      int id = page_of(0);
-      for (int j = 0; ok && j < w.nkv; ++j) {
+      int ids = fetch_ids(0);
+      for (int j = 0; j < w.nkv; ++j) {
         const int s = j % NS;
-        const int next = page_of(j + 1);
-        if (j >= NS && !mbar_wait_warp(&kv_empty[s], ((j / NS) - 1) & 1, 0x501)) break;
-        const int key0 = key0_of(j), row = (key0 + lane * box) & ((1 << p.bs_log2) - 1);
-        const uint32_t have = __ballot_sync(0xffffffffu, id >= 0);  // bit per box
+        const int next = fetch_ids(j + 1);
+        const int key0 = key0_of(j), key = key0 + lane * box, row = key & ((1 << p.bs_log2) - 1);
+        int id = __shfl_sync(0xffffffffu, ids, (lane * box >> 3) & 15);
+        if (lane < per_tile && !any_seen(key, box)) id = -1;
+        // Eight-row groups of the cache; one past its end reads as zeros.
+        const int at = id >= 0 ? (int)((((int64_t)id * p.Hkv + w.hk) << (p.bs_log2 - 3)) + (row >> 3))
+                               : (int)(((int64_t)p.num_blocks * p.Hkv) << (p.bs_log2 - 3));
         const bool clean = all_seen_by_some(key0, BN);
-        if (lane == 0) {
-          uint32_t m = 0;  // bit per 8 keys
-          for (int b = 0; b < per_tile; ++b)
-            if ((have >> b) & 1) m |= ((1u << (box / 8)) - 1u) << (b * (box / 8));
-          pages[s] = m;
-          mbar_arrive_expect_tx(&k_full[s], KC * CHUNK_BYTES);
-          mbar_arrive_expect_tx(clean ? &v_full[s] : edge, KC * CHUNK_BYTES);
-        }
-        __syncwarp();
-        // A block past the cache reads as zeros.
-        const int blk = id >= 0 ? id : p.num_blocks;
-        if (lane < per_tile)
-          for (int kc = 0; kc < KC; ++kc)
-            tma_load_4d(sK + (s * KC + kc) * CHUNK_BYTES + lane * box * 128, &tk, &k_full[s], kc * 64,
-                        row, w.hk, blk);
+        if (j >= NS && !mbar_wait_warp(&k_empty[s], ((j / NS) - 1) & 1, 0x501)) break;
+        if (lane == 0) mbar_arrive_expect_tx(&k_full[s], L::TILE);
         __syncwarp();
         if (lane < per_tile)
-          for (int kc = 0; kc < KC; ++kc)
-            tma_load_4d(sV + (s * KC + kc) * CHUNK_BYTES + lane * box * 128, &tv,
-                        clean ? &v_full[s] : edge, kc * 64, row, w.hk, blk);
+          tma_load_4d(sK + s * L::TILE + lane * box * (KC * 128), &tk, &k_full[s], 0, 0, 0, at);
+        if (j >= NS && !mbar_wait_warp(&v_empty[s], ((j / NS) - 1) & 1, 0x503)) break;
+        if (lane == 0) mbar_arrive_expect_tx(clean ? &v_full[s] : edge, L::TILE);
+        __syncwarp();
+        if (lane < per_tile)
+          tma_load_4d(sV + s * L::TILE + lane * box * (KC * 128), &tv, clean ? &v_full[s] : edge, 0, 0,
+                      0, at);
         if (!clean) {
           if (!mbar_wait_warp(edge, edges & 1, 0x502)) break;
           ++edges;
@@ -274,18 +278,18 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             if (!seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key0 + r))
               for (int kc = 0; kc < KC; ++kc)
                 for (int c = 0; c < 8; ++c)
-                  *reinterpret_cast<uint4*>(sV + (s * KC + kc) * CHUNK_BYTES + r * 128 + c * 16) =
-                      make_uint4(0u, 0u, 0u, 0u);
+                  *reinterpret_cast<uint4*>(sV + s * L::TILE + ((r >> 3) * KC + kc) * ATOM + (r & 7) * 128 +
+                                            c * 16) = make_uint4(0u, 0u, 0u, 0u);
           fence_async_shared();
           __syncwarp();
           if (lane == 0) mbar_arrive(&v_full[s]);
         }
-        id = next;
+        ids = next;
       }
     }
   } else if (warp == 1) {
     // --------------------------------------------------------- MMA issue --
-    reg_dealloc<FP8 ? 56 : 96>();
+    reg_dealloc<FP8 ? 48 : 96>();
     if (lane == 0) {
       constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, FMT, 0, 0);
       constexpr uint32_t IDESC_PV = idesc_f16(BM, D, FMT, 0, 1);
@@ -294,9 +298,9 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         const int s = j % NS;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * CHUNK_BYTES + (kk % 4) * 32;
-          mma_ss(tmem + t * 128, smem_desc_sw128(q_base + t * KC * CHUNK_BYTES + off, 16, 1024),
-                 smem_desc_sw128(k_base + s * KC * CHUNK_BYTES + off, 16, 1024), IDESC_QK, kk > 0);
+          const uint32_t qo = (kk / 4) * CHUNK_BYTES + (kk % 4) * 32, ko = (kk / 4) * ATOM + (kk % 4) * 32;
+          mma_ss(tmem + t * 128, smem_desc_sw128(q_base + t * KC * CHUNK_BYTES + qo, 16, ATOM),
+                 smem_desc_sw128(k_base + s * L::TILE + ko, 16, KC * ATOM), IDESC_QK, kk > 0);
         }
         mma_commit(&s_full[t]);
       };
@@ -307,7 +311,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         for (int k4 = 0; k4 < BN / 32; ++k4) {
           const int kk = h * (BN / 32) + k4;
           mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
-                 smem_desc_sw128(v_base + s * KC * CHUNK_BYTES + kk * 2048, CHUNK_BYTES, 1024),
+                 smem_desc_sw128(v_base + s * L::TILE + kk * (2 * KC * ATOM), ATOM, KC * ATOM),
                  IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
         }
         if (h == 1) mma_commit(&pv_done[t]);
@@ -319,6 +323,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       tc_fence_after();
       for (int t = 0; ok && t < TILES; ++t)
         if (w.nkv_t[t] > 0) issue_qk(t, 0);
+      if (ok && w.nkv > 0) mma_commit(&k_empty[0]);
       for (int j = 0; ok && j < w.nkv; ++j) {
         const int s = j % NS;
         if (!mbar_wait(&v_full[s], (j / NS) & 1, 0x513)) { ok = false; break; }
@@ -336,14 +341,16 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             issue_qk(t, j + 1);
           }
         }
-        if (ok) mma_commit(&kv_empty[s]);
+        if (!ok) break;
+        mma_commit(&v_empty[s]);
+        if (j + 1 < w.nkv) mma_commit(&k_empty[(j + 1) % NS]);
       }
     }
   } else if (warp < 4) {
-    reg_dealloc<FP8 ? 56 : 96>();  // idle members of the first warpgroup
+    reg_dealloc<FP8 ? 48 : 96>();  // idle members of the first warpgroup
   } else if (warp < 12) {
     // ----------------------------------------------------------- softmax --
-    reg_alloc<FP8 ? 184 : 200>();
+    reg_alloc<FP8 ? 136 : 200>();
     const int t = (warp >> 2) - 1;
     const int row = threadIdx.x - 128 * (t + 1);  // TMEM lane
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -356,24 +363,19 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     if ((w.c0 + t) * w.R < w.pairs) tile_positions(p, w.q, w.c0 + t, w.R, tile_lo, tile_hi);
     float m = -INFINITY, l = 0.f;
     bool ok = true;
+    int ids = fetch_ids(0);
     for (int j = 0; j < nkv_t; ++j) {
-      const int s = j % NS;
-      // (k_full has long completed: its wait orders the reads of `pages`.)
-      if (!mbar_wait_warp(&s_full[t], j & 1, 0x521) ||
-          !mbar_wait_warp(&k_full[s], (j / NS) & 1, 0x522)) { ok = false; break; }
+      const uint32_t have = __ballot_sync(0xffffffffu, ids >= 0);  // bit per 8 keys: page there
+      ids = fetch_ids(j + 1);
+      if (!mbar_wait_warp(&s_full[t], j & 1, 0x521)) { ok = false; break; }
       tc_fence_after();
-      uint32_t sr[4][32];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(lane_addr + t * 128 + 32 * i, sr[i]);
-      const uint32_t have = pages[s];
-      const int kv0 = key0_of(j);
-      tmem_ld_wait();
-      const int last = kv0 + BN - 1;
+      const int kv0 = key0_of(j), last = kv0 + BN - 1;
       const bool whole = last <= tile_lo && last < w.q.ctx && have == 0xffffu &&
                          (p.window == 0 || tile_hi - kv0 < p.window || last < p.sinks);
+      // Visible columns as bits, 32 columns a word: below hi, from lo on (or a
+      // sink, below sk), and in a page that is there.
+      uint32_t bits[4];
       if (!whole) {
-        // Visible columns as bits, 32 columns a word: below hi, from lo on (or a
-        // sink, below sk), and in a page that is there.
         const int hi = min(w.q.ctx, pos + 1) - kv0;
         const int lo = p.window > 0 ? pos - p.window + 1 - kv0 : 0;
         const int sk = p.window > 0 ? p.sinks - kv0 : 0;
@@ -382,14 +384,49 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           uint32_t pg = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b) pg |= (0u - ((have >> (4 * i + b)) & 1u)) & (0xffu << (8 * b));
-          const uint32_t bits =
-              low_bits(hi - 32 * i) & (~low_bits(lo - 32 * i) | low_bits(sk - 32 * i)) & pg;
-#pragma unroll
-          for (int cc = 0; cc < 32; ++cc)
-            if (!((bits >> cc) & 1)) sr[i][cc] = __float_as_uint(-INFINITY);
+          bits[i] = low_bits(hi - 32 * i) & (~low_bits(lo - 32 * i) | low_bits(sk - 32 * i)) & pg;
         }
       }
-      const float mx = row_max(sr);
+      // Scores of columns [32 i, 32 i + 32), hidden ones at -inf (after the wait).
+      auto fetch = [&](int i, uint32_t (&x)[32]) { tmem_ld32(lane_addr + t * 128 + 32 * i, x); };
+      auto hide = [&](int i, uint32_t (&x)[32]) {
+#pragma unroll
+        for (int cc = 0; cc < 32; ++cc)
+          if (!((bits[i] >> cc) & 1)) x[cc] = __float_as_uint(-INFINITY);
+      };
+      // 16-bit cache: all 128 scores stay in registers. e4m3: the converter
+      // warpgroups leave room for 64; columns [64, 128) are read once for the
+      // maximum and again after the first half's exponentials.
+      constexpr int HELD = FP8 ? 2 : 4;
+      uint32_t sr[HELD][32];
+      float mx;
+      if constexpr (FP8) {
+        fetch(2, sr[0]);
+        fetch(3, sr[1]);
+        tmem_ld_wait();
+        if (!whole) {
+          hide(2, sr[0]);
+          hide(3, sr[1]);
+        }
+        mx = row_max(sr);
+        fetch(0, sr[0]);
+        fetch(1, sr[1]);
+        tmem_ld_wait();
+        if (!whole) {
+          hide(0, sr[0]);
+          hide(1, sr[1]);
+        }
+        mx = fmaxf(mx, row_max(sr));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fetch(i, sr[i]);
+        tmem_ld_wait();
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) hide(i, sr[i]);
+        }
+        mx = row_max(sr);
+      }
       const float m_new = fmaxf(m, mx * sl2);
       float alpha = 1.f;
       const bool rescale = m_new > m + RESCALE_THRESHOLD;
@@ -402,24 +439,36 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                       make_float2(0.f, 0.f)};
       const float2 sl2_2 = make_float2(sl2, sl2), negm2 = make_float2(-m_use, -m_use);
+      auto weigh = [&](const uint32_t (&x)[32], uint32_t* pk) {  // 32 scores to 16 packed pairs
+#pragma unroll
+        for (int cc = 0; cc < 16; ++cc) {
+          const float2 y = __ffma2_rn(
+              make_float2(__uint_as_float(x[2 * cc]), __uint_as_float(x[2 * cc + 1])), sl2_2, negm2);
+          const float2 pp = make_float2(ex2(y.x), ex2(y.y));
+          l2[cc & 3] = __fadd2_rn(l2[cc & 3], pp);
+          pk[cc] = FMT == 1 ? pack_bf16(pp.x, pp.y) : pack_f16(pp.x, pp.y);
+        }
+      };
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int i = 2 * h; i < 2 * h + 2; ++i) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int cc = 0; cc < 16; ++cc) {
-            const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[i][2 * cc]),
-                                                    __uint_as_float(sr[i][2 * cc + 1])),
-                                        sl2_2, negm2);
-            const float2 pp = make_float2(ex2(x.x), ex2(x.y));
-            l2[cc & 3] = __fadd2_rn(l2[cc & 3], pp);
-            pk[cc] = FMT == 1 ? pack_bf16(pp.x, pp.y) : pack_f16(pp.x, pp.y);
+        uint32_t pk[32];
+        if constexpr (FP8) {
+          if (h == 1) {
+            fetch(2, sr[0]);
+            fetch(3, sr[1]);
+            tmem_ld_wait();
+            if (!whole) {
+              hide(2, sr[0]);
+              hide(3, sr[1]);
+            }
           }
-#pragma unroll
-          for (int cc = 0; cc < 16; ++cc) sr[h][(i & 1) * 16 + cc] = pk[cc];
+          weigh(sr[0], pk);
+          weigh(sr[1], pk + 16);
+        } else {
+          weigh(sr[2 * h], pk);
+          weigh(sr[2 * h + 1], pk + 16);
         }
-        tmem_st32(lane_addr + t * 128 + 32 * h, sr[h]);
+        tmem_st32(lane_addr + t * 128 + 32 * h, pk);
         // O is rescaled before the first half's PV accumulates into it; PV_t(j-1)
         // has completed: s_full(j) follows it in issue order.
         if (h == 0 && __any_sync(0xffffffffu, rescale && j > 0)) {
@@ -496,29 +545,23 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     }
   } else {
     // ----------------------------------------------------------- convert --
-    reg_dealloc<88>();
+    reg_dealloc<80>();
     if constexpr (FP8) {
       constexpr int CPR = D / 16;           // 16-byte pieces of a cached row
       constexpr int RPP = 128 / CPR;        // rows per pass of the 128 threads
       constexpr int PASSES = BN / RPP;
-      const int tid = threadIdx.x - 384, c = tid % CPR, r0 = tid / CPR;
+      const bool is_v = warp >= 16;         // 12-15 convert K, 16-19 V
+      const int tid = threadIdx.x & 127, c = tid % CPR, r0 = tid / CPR;
       const int bs = 1 << p.bs_log2;
-      // Page ids of a tile, lane b < 16 holding that of keys [8 b, 8 b + 8) (-1:
-      // none), fetched a tile ahead of the rows they lead to.
-      auto fetch_ids = [&](int j) -> int {
-        if (lane >= BN / 8 || j >= w.nkv) return -1;
-        const int key = key0_of(j) + 8 * lane;
-        if (key >= w.q.ctx) return -1;
-        const int id = bt[key >> p.bs_log2];
-        return id >= 0 && id < p.num_blocks ? id : -1;
-      };
       // Registers of one tile: 16 bytes and a scale of rows r0, r0 + RPP, ...;
       // rows that no row of the item sees, or whose page is missing, are zeros.
       struct Tile {
         uint4 x[PASSES];
         uint32_t e[PASSES];
       };
-      auto load = [&](Tile& r, const uint8_t* cache, const uint8_t* scale, int j, int ids) {
+      const uint8_t* cache = static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache);
+      const uint8_t* scale = is_v ? p.v_scale : p.k_scale;
+      auto load = [&](Tile& r, int j, int ids) {
         const int key0 = key0_of(j);
         const bool clean = all_seen_by_some(key0, BN);
 #pragma unroll
@@ -560,7 +603,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
               }
             }
           }
-          uint8_t* base = tile + kc * CHUNK_BYTES + row * 128;
+          uint8_t* base = tile + ((row >> 3) * KC + kc) * ATOM + (row & 7) * 128;
           // Halves in alternating order, so that 8 lanes of a row touch every bank once.
           const int first = (c >> 2) & 1, piece = (c & 3) * 2;
           const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
@@ -568,30 +611,22 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           *reinterpret_cast<uint4*>(base + (((piece + 1 - first) ^ (row & 7)) << 4)) = first ? lo : hi;
         }
       };
-      bool ok = true;
-      const uint8_t* kc = static_cast<const uint8_t*>(p.k_cache);
-      const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache);
-      Tile kt, vt;
+      uint8_t* tiles = is_v ? sV : sK;
+      uint64_t* full = is_v ? v_full : k_full;
+      uint64_t* empty = is_v ? v_empty : k_empty;
+      Tile x;
       int ids = fetch_ids(0), next = fetch_ids(1);
-      if (w.nkv > 0) load(kt, kc, p.k_scale, 0, ids);
+      if (w.nkv > 0) load(x, 0, ids);
       for (int j = 0; j < w.nkv; ++j) {
         const int s = j % NS;
-        load(vt, vc, p.v_scale, j, ids);
-        if (j >= NS && !mbar_wait_warp(&kv_empty[s], ((j / NS) - 1) & 1, 0x531)) break;
-        // Pages by 8 keys, for the softmax warps (ordered by this warp's arrival).
-        const uint32_t have = __ballot_sync(0xffffffffu, ids >= 0);
-        if (tid == 0) pages[s] = have;
+        if (j >= NS && !mbar_wait_warp(&empty[s], ((j / NS) - 1) & 1, 0x531)) break;
         ids = next;
         next = fetch_ids(j + 2);
-        store(kt, sK + s * KC * CHUNK_BYTES);
+        store(x, tiles + s * L::TILE);
+        if (j + 1 < w.nkv) load(x, j + 1, ids);
         fence_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[s]);
-        if (j + 1 < w.nkv) load(kt, kc, p.k_scale, j + 1, ids);
-        store(vt, sV + s * KC * CHUNK_BYTES);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[s]);
+        if (lane == 0) mbar_arrive(&full[s]);
       }
     }
   }
@@ -628,16 +663,37 @@ static int make_q_map(CUtensorMap* map, const Params& p, int dtype) {
   return LSB_OK;
 }
 
+// The cache as [rows / 8, D / 64, 8, 64]: a box is `groups` row groups of one page.
+static int make_cache_map(CUtensorMap* map, const void* base, const Params& p, int dtype, int groups) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled unavailable (no CUDA driver?)");
+    return LSB_ERR_CUDA;
+  }
+  const int64_t rows8 = ((int64_t)p.num_blocks * p.Hkv) << (p.bs_log2 - 3);
+  cuuint64_t dims[4] = {64, 8, (cuuint64_t)(p.D / 64), (cuuint64_t)rows8};
+  cuuint64_t strides[3] = {(cuuint64_t)p.D * 2, 128, (cuuint64_t)p.D * 16};
+  cuuint32_t box[4] = {64, 8, (cuuint32_t)(p.D / 64), (cuuint32_t)groups};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, dtype == LSB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                   4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LSB_ERR_CUDA;
+  }
+  return LSB_OK;
+}
+
 template <int D, int FMT, bool FP8>
 static int launch(const Params& p, int dtype, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   int rc = make_q_map(&mq, p, dtype);
   const int box_log2 = std::min(p.bs_log2, 7);
-  const int64_t bs = 1LL << p.bs_log2;
-  const int64_t sc[4] = {(int64_t)p.Hkv * bs * D, bs * D, D, 1};  // [num_blocks, Hkv, bs, D]
   if (!FP8) {
-    if (!rc) rc = make_bhnd_map(&mk, p.k_cache, dtype, p.num_blocks, p.Hkv, bs, D, sc, 64, 1u << box_log2);
-    if (!rc) rc = make_bhnd_map(&mv, p.v_cache, dtype, p.num_blocks, p.Hkv, bs, D, sc, 64, 1u << box_log2);
+    if (!rc) rc = make_cache_map(&mk, p.k_cache, p, dtype, 1 << (box_log2 - 3));
+    if (!rc) rc = make_cache_map(&mv, p.v_cache, p, dtype, 1 << (box_log2 - 3));
   } else {
     mk = mv = mq;  // not used
   }
@@ -647,7 +703,7 @@ static int launch(const Params& p, int dtype, cudaStream_t st) {
   if (int rc_ = limit.ensure(kern, Smem<D>::ALLOC, "paged_attn smem attribute")) return rc_;
   const int64_t R = (int64_t)(BM / p.G * p.G) * TILES;
   const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)(((int64_t)p.max_q * p.G + R - 1) / R), (unsigned)p.S);
-  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(FP8 ? 512 : 384), Smem<D>::ALLOC, st, mq, mk, mv, p, box_log2),
+  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(FP8 ? 640 : 384), Smem<D>::ALLOC, st, mq, mk, mv, p, box_log2),
               "paged_attn");
   return LSB_OK;
 }
@@ -664,6 +720,8 @@ bool tc_eligible(const Params& p, int dtype, bool kv_fp8) {
   if (!aligned16(p.k_cache) || !aligned16(p.v_cache)) return false;
   if (p.T > 1 && p.sq_t == 0) return false;
   if (p.Hq > 1 && p.sq_h == 0) return false;
+  // The cache's 8-row groups are a 32-bit TMA coordinate.
+  if ((((int64_t)p.num_blocks * p.Hkv) << (p.bs_log2 - 3)) > 0x7fffffff) return false;
   const int64_t R = (int64_t)(tc::BM / p.G * p.G) * tc::TILES;
   return ((int64_t)p.max_q * p.G + R - 1) / R <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff;
 }
