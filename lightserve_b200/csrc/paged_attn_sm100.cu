@@ -12,11 +12,9 @@
 //    8-row groups, so the box's atoms land as the MMA's descriptors want them; a
 //    box per 64-column half took 13% longer over pages of 16). Pages that do not
 //    exist, or that no row sees, are fetched past the end: zeros.
-//  * e4m3 cache: two converter warpgroups, for K and V, read the rows (16 bytes a
-//    thread, one tile ahead in registers), multiply by the row's power of two in
-//    fp32 and round to q's type, which is exact in bf16 (and in fp16 within its
-//    range), and write the swizzled tiles, in the shadow of the S -> softmax -> P
-//    chain that bounds the kernel.
+//  * e4m3 cache: TMA stages the raw tile, and two converter warpgroups, for K and
+//    V, multiply each row by its power of two in fp32, round to q's type (exact in
+//    bf16, and in fp16 within its range) and write the swizzled tiles.
 //  * V rows that no row of the item sees (past the context, between sinks and
 //    window) are zeroed in shared memory, so that what such cells hold never
 //    meets a weight of 0; the tiles that need it are the ends of a span.
@@ -52,17 +50,20 @@ constexpr int CHUNK_BYTES = 128 * 128;  // Q: [128 rows][64 columns] of 16 bits
 constexpr int ATOM = 1024;
 constexpr float RESCALE_THRESHOLD = 8.0f;
 
-template <int D>
+template <int D, bool FP8>
 struct Smem {
   static constexpr int KC = D / 64;
   static constexpr int TILE = KC * CHUNK_BYTES;  // bytes of a K or V tile
+  static constexpr int RAW = BN * D;             // bytes of an e4m3 tile
   static constexpr int Q_OFF = 0;
   static constexpr int K_OFF = Q_OFF + TILES * KC * CHUNK_BYTES;
   static constexpr int V_OFF = K_OFF + NS * KC * CHUNK_BYTES;
-  static constexpr int BAR_OFF = V_OFF + NS * KC * CHUNK_BYTES;
+  static constexpr int RAW_OFF = V_OFF + NS * KC * CHUNK_BYTES;  // e4m3 K, V, then their scales
+  static constexpr int SCALE_OFF = RAW_OFF + (FP8 ? 2 * RAW : 0);
+  static constexpr int BAR_OFF = SCALE_OFF + (FP8 ? 2 * BN : 0);
   // q_full[2], k_full[NS], v_full[NS], k_empty[NS], v_empty[NS], s_full[2], p_full[2][2],
-  // pv_done[2], edge
-  static constexpr int NBAR = TILES + 4 * NS + 4 * TILES + 1;
+  // pv_done[2], edge, raw_full[2], raw_empty[2]
+  static constexpr int NBAR = TILES + 4 * NS + 4 * TILES + 1 + 4;
   static constexpr int TMEM_SLOT_OFF = BAR_OFF + NBAR * 8;
   static constexpr int BYTES = TMEM_SLOT_OFF + 16;
   static constexpr int ALLOC = BYTES + 1024;  // slack for 1024-byte alignment
@@ -87,6 +88,15 @@ __device__ __forceinline__ void fence_async_shared() {
 // The n lowest bits set (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u;
+}
+
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0,
+                                            int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
 }
 
 template <int N>
@@ -152,7 +162,7 @@ template <int D, int FMT, bool FP8>
 __global__ void __launch_bounds__(FP8 ? 640 : 384, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const Params p, const int box_log2) {
-  using L = Smem<D>;
+  using L = Smem<D, FP8>;
   using T = typename std::conditional<FMT == 1, __nv_bfloat16, __half>::type;
   constexpr int KC = L::KC;
   extern __shared__ uint8_t smem_raw[];
@@ -169,6 +179,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   uint64_t* p_full = s_full + TILES;      // [TILES][2]
   uint64_t* pv_done = p_full + 2 * TILES; // [TILES]
   uint64_t* edge = pv_done + TILES;       // V boxes of a tile that is zeroed in places
+  uint64_t* raw_full = edge + 1;          // [K, V]: the e4m3 tile is in shared memory
+  uint64_t* raw_empty = raw_full + 2;     // [K, V]: its converters have read it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::TMEM_SLOT_OFF);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -192,6 +204,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       mbar_init(&v_empty[s], 1);
     }
     mbar_init(edge, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
+    }
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -285,6 +301,45 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           if (lane == 0) mbar_arrive(&v_full[s]);
         }
         ids = next;
+      }
+    } else {
+      const int box = 1 << box_log2, per_tile = BN >> box_log2;
+      // Scales of 8 keys a lane (0-15 of K, 16-31 of V), a tile ahead; their page
+      // ids two.
+      auto fetch_scales = [&](int j, int ids) -> uint2 {
+        const int id = __shfl_sync(0xffffffffu, ids, lane & 15);
+        if (id < 0) return make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+        const int key = key0_of(j) + 8 * (lane & 15);
+        const int64_t cell = (((int64_t)id * p.Hkv + w.hk) << p.bs_log2) + (key & ((1 << p.bs_log2) - 1));
+        return __ldg(reinterpret_cast<const uint2*>((lane < 16 ? p.k_scale : p.v_scale) + cell));
+      };
+      int ids = fetch_ids(0), ids1 = fetch_ids(1);
+      uint2 sc = fetch_scales(0, ids);
+      for (int j = 0; j < w.nkv; ++j) {
+        const int ids2 = fetch_ids(j + 2);
+        const uint2 sc1 = fetch_scales(j + 1, ids1);
+        const int key = key0_of(j) + lane * box;
+        int id = __shfl_sync(0xffffffffu, ids, (lane * box >> 3) & 15);
+        if (lane < per_tile && !any_seen(key, box)) id = -1;
+        // Rows of the cache; one past its end reads as zeros.
+        const int at = (int)((((int64_t)(id >= 0 ? id : p.num_blocks) * p.Hkv + (id >= 0 ? w.hk : 0))
+                              << p.bs_log2) + (id >= 0 ? key & ((1 << p.bs_log2) - 1) : 0));
+        bool ok = true;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (j > 0 && !mbar_wait_warp(&raw_empty[kv], (j - 1) & 1, 0x504)) { ok = false; break; }
+          if (lane >> 4 == kv) *reinterpret_cast<uint2*>(smem + L::SCALE_OFF + lane * 8) = sc;
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(&raw_full[kv], L::RAW);
+          __syncwarp();
+          if (lane < per_tile)
+            tma_load_2d(smem + L::RAW_OFF + kv * L::RAW + lane * box * D, kv == 0 ? &tk : &tv,
+                        &raw_full[kv], 0, at);
+        }
+        if (!ok) break;
+        ids = ids1;
+        ids1 = ids2;
+        sc = sc1;
       }
     }
   } else if (warp == 1) {
@@ -552,78 +607,65 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       constexpr int PASSES = BN / RPP;
       const bool is_v = warp >= 16;         // 12-15 convert K, 16-19 V
       const int tid = threadIdx.x & 127, c = tid % CPR, r0 = tid / CPR;
-      const int bs = 1 << p.bs_log2;
-      // Registers of one tile: 16 bytes and a scale of rows r0, r0 + RPP, ...;
-      // rows that no row of the item sees, or whose page is missing, are zeros.
-      struct Tile {
-        uint4 x[PASSES];
-        uint32_t e[PASSES];
-      };
-      const uint8_t* cache = static_cast<const uint8_t*>(is_v ? p.v_cache : p.k_cache);
-      const uint8_t* scale = is_v ? p.v_scale : p.k_scale;
-      auto load = [&](Tile& r, int j, int ids) {
-        const int key0 = key0_of(j);
-        const bool clean = all_seen_by_some(key0, BN);
+      // A thread's rows r0, r0 + RPP, ... of the tile, 16 bytes of each. Rows that
+      // no row of the item sees become zeros (missing pages arrived as such).
+      auto store = [&](int i, const uint4& raw16, int scale, uint8_t* tile) {
+        const int kc = c / 4, row = r0 + i * RPP;
+        const float f = e8m0_to_float(scale);
+        const uint32_t words[4] = {raw16.x, raw16.y, raw16.z, raw16.w};
+        uint32_t o[8];
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          const int row = r0 + i * RPP, key = key0 + row;
-          const int id = __shfl_sync(0xffffffffu, ids, row >> 3);
-          const bool ok = id >= 0 && (clean || seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key));
-          const int64_t cell = ((int64_t)max(id, 0) * p.Hkv + w.hk) * bs + (key & (bs - 1));
-          r.x[i] = make_uint4(0u, 0u, 0u, 0u);
-          r.e[i] = 127;
-          if (ok) {
-            r.x[i] = __ldg(reinterpret_cast<const uint4*>(cache + cell * D) + c);
-            r.e[i] = __ldg(scale + cell);
-          }
-        }
-      };
-      auto store = [&](const Tile& r, uint8_t* tile) {
-        const int kc = c / 4;
+        for (int q4 = 0; q4 < 4; ++q4) {
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          const int row = r0 + i * RPP;
-          const float f = e8m0_to_float((int)r.e[i]);
-          const uint32_t words[4] = {r.x[i].x, r.x[i].y, r.x[i].z, r.x[i].w};
-          uint32_t o[8];
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float2 y = __fmul2_rn(
-                  f16x2_to_float2(cvt_e4m3x2_f16x2((uint16_t)(words[q4] >> (16 * e)))), make_float2(f, f));
-              if constexpr (FMT == 1) {
-                o[2 * q4 + e] = pack_bf16(y.x, y.y);
-              } else {  // a value lifted past fp16's range stays at its largest
-                const __half2 top = __float2half2_rn(65504.f);
-                const uint32_t z = pack_f16(y.x, y.y);
-                const __half2 c2 = __hmax2_nan(
-                    __hmin2_nan(*reinterpret_cast<const __half2*>(&z), top), __hneg2(top));
-                o[2 * q4 + e] = *reinterpret_cast<const uint32_t*>(&c2);
-              }
+          for (int e = 0; e < 2; ++e) {
+            const float2 y = __fmul2_rn(
+                f16x2_to_float2(cvt_e4m3x2_f16x2((uint16_t)(words[q4] >> (16 * e)))), make_float2(f, f));
+            if constexpr (FMT == 1) {
+              o[2 * q4 + e] = pack_bf16(y.x, y.y);
+            } else {  // a value lifted past fp16's range stays at its largest
+              const __half2 top = __float2half2_rn(65504.f);
+              const uint32_t z = pack_f16(y.x, y.y);
+              const __half2 c2 =
+                  __hmax2_nan(__hmin2_nan(*reinterpret_cast<const __half2*>(&z), top), __hneg2(top));
+              o[2 * q4 + e] = *reinterpret_cast<const uint32_t*>(&c2);
             }
           }
-          uint8_t* base = tile + ((row >> 3) * KC + kc) * ATOM + (row & 7) * 128;
-          // Halves in alternating order, so that 8 lanes of a row touch every bank once.
-          const int first = (c >> 2) & 1, piece = (c & 3) * 2;
-          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-          *reinterpret_cast<uint4*>(base + (((piece + first) ^ (row & 7)) << 4)) = first ? hi : lo;
-          *reinterpret_cast<uint4*>(base + (((piece + 1 - first) ^ (row & 7)) << 4)) = first ? lo : hi;
         }
+        uint8_t* base = tile + ((row >> 3) * KC + kc) * ATOM + (row & 7) * 128;
+        // Halves in alternating order, so that 8 lanes of a row touch every bank once.
+        const int first = (c >> 2) & 1, piece = (c & 3) * 2;
+        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+        *reinterpret_cast<uint4*>(base + (((piece + first) ^ (row & 7)) << 4)) = first ? hi : lo;
+        *reinterpret_cast<uint4*>(base + (((piece + 1 - first) ^ (row & 7)) << 4)) = first ? lo : hi;
       };
       uint8_t* tiles = is_v ? sV : sK;
       uint64_t* full = is_v ? v_full : k_full;
       uint64_t* empty = is_v ? v_empty : k_empty;
-      Tile x;
-      int ids = fetch_ids(0), next = fetch_ids(1);
-      if (w.nkv > 0) load(x, 0, ids);
+      const uint8_t* raw = smem + L::RAW_OFF + is_v * L::RAW;
+      const uint8_t* scales = smem + L::SCALE_OFF + is_v * BN;
       for (int j = 0; j < w.nkv; ++j) {
-        const int s = j % NS;
-        if (j >= NS && !mbar_wait_warp(&empty[s], ((j / NS) - 1) & 1, 0x531)) break;
-        ids = next;
-        next = fetch_ids(j + 2);
-        store(x, tiles + s * L::TILE);
-        if (j + 1 < w.nkv) load(x, j + 1, ids);
+        const int s = j % NS, key0 = key0_of(j);
+        if (!mbar_wait_warp(&raw_full[is_v], j & 1, 0x531)) break;
+        uint4 x[PASSES];
+        int e[PASSES];
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+          x[i] = *reinterpret_cast<const uint4*>(raw + (r0 + i * RPP) * D + c * 16);
+          e[i] = scales[r0 + i * RPP];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_empty[is_v]);  // the next tile may come
+        if (!all_seen_by_some(key0, BN)) {
+#pragma unroll
+          for (int i = 0; i < PASSES; ++i)
+            if (!seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key0 + r0 + i * RPP)) {
+              x[i] = make_uint4(0u, 0u, 0u, 0u);
+              e[i] = 127;
+            }
+        }
+        if (j >= NS && !mbar_wait_warp(&empty[s], ((j / NS) - 1) & 1, 0x532)) break;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) store(i, x[i], e[i], tiles + s * L::TILE);
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[s]);
@@ -686,6 +728,27 @@ static int make_cache_map(CUtensorMap* map, const void* base, const Params& p, i
   return LSB_OK;
 }
 
+// An e4m3 cache as [rows, D] bytes: a box is the rows of a page.
+static int make_raw_map(CUtensorMap* map, const void* base, const Params& p, int rows_per_box) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled unavailable (no CUDA driver?)");
+    return LSB_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)p.D, (cuuint64_t)(((int64_t)p.num_blocks * p.Hkv) << p.bs_log2)};
+  cuuint64_t strides[1] = {(cuuint64_t)p.D};
+  cuuint32_t box[2] = {(cuuint32_t)p.D, (cuuint32_t)rows_per_box};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LSB_ERR_CUDA;
+  }
+  return LSB_OK;
+}
+
 template <int D, int FMT, bool FP8>
 static int launch(const Params& p, int dtype, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
@@ -695,15 +758,16 @@ static int launch(const Params& p, int dtype, cudaStream_t st) {
     if (!rc) rc = make_cache_map(&mk, p.k_cache, p, dtype, 1 << (box_log2 - 3));
     if (!rc) rc = make_cache_map(&mv, p.v_cache, p, dtype, 1 << (box_log2 - 3));
   } else {
-    mk = mv = mq;  // not used
+    if (!rc) rc = make_raw_map(&mk, p.k_cache, p, 1 << box_log2);
+    if (!rc) rc = make_raw_map(&mv, p.v_cache, p, 1 << box_log2);
   }
   if (rc) return rc;
   auto kern = paged_chunk_kernel<D, FMT, FP8>;
   static SmemLimit limit;
-  if (int rc_ = limit.ensure(kern, Smem<D>::ALLOC, "paged_attn smem attribute")) return rc_;
+  if (int rc_ = limit.ensure(kern, Smem<D, FP8>::ALLOC, "paged_attn smem attribute")) return rc_;
   const int64_t R = (int64_t)(BM / p.G * p.G) * TILES;
   const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)(((int64_t)p.max_q * p.G + R - 1) / R), (unsigned)p.S);
-  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(FP8 ? 640 : 384), Smem<D>::ALLOC, st, mq, mk, mv, p, box_log2),
+  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(FP8 ? 640 : 384), Smem<D, FP8>::ALLOC, st, mq, mk, mv, p, box_log2),
               "paged_attn");
   return LSB_OK;
 }
@@ -720,8 +784,11 @@ bool tc_eligible(const Params& p, int dtype, bool kv_fp8) {
   if (!aligned16(p.k_cache) || !aligned16(p.v_cache)) return false;
   if (p.T > 1 && p.sq_t == 0) return false;
   if (p.Hq > 1 && p.sq_h == 0) return false;
-  // The cache's 8-row groups are a 32-bit TMA coordinate.
-  if ((((int64_t)p.num_blocks * p.Hkv) << (p.bs_log2 - 3)) > 0x7fffffff) return false;
+  // The cache's 8-row groups (e4m3: rows) are a 32-bit TMA coordinate; scales are
+  // read 8 keys at a time.
+  if ((((int64_t)p.num_blocks * p.Hkv) << (kv_fp8 ? p.bs_log2 : p.bs_log2 - 3)) > 0x7fffffff) return false;
+  if (kv_fp8 && ((reinterpret_cast<uintptr_t>(p.k_scale) | reinterpret_cast<uintptr_t>(p.v_scale)) & 7))
+    return false;
   const int64_t R = (int64_t)(tc::BM / p.G * p.G) * tc::TILES;
   return ((int64_t)p.max_q * p.G + R - 1) / R <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff;
 }
