@@ -73,9 +73,9 @@ __device__ __forceinline__ float finite_abs(float x) {
 // infinity, and the conversion would saturate them to 448).
 __device__ __forceinline__ float scaled_for_e4m3(float x, float inv) { return fmaf(x, inv, x - x); }
 
-// Dequantised value in T. Rounding to e4m3 can lift a value at the top of
-// T's range past it (65504 becomes 65536): the result stays at T's largest
-// finite value. NaN stays NaN.
+// Rounding to e4m3 can lift a value at the top of T's range past it (65504
+// becomes 65536): a dequantised row, and an attention output made of such
+// values, stays at T's largest finite value. NaN stays NaN.
 template <typename T> struct FiniteMax;
 template <> struct FiniteMax<float> { static constexpr float v = 3.402823466e38f; };
 template <> struct FiniteMax<__nv_bfloat16> { static constexpr float v = 3.38953139e38f; };

@@ -190,7 +190,7 @@ paged_simt_kernel(const Params p, const bool vec) {
       T* dst = static_cast<T*>(p.o) + (int64_t)row * p.so_t + (int64_t)h * p.so_h;
 #pragma unroll
       for (int c = 0; c < DC; ++c)
-        if (c * 32 + lane < D) dst[c * 32 + lane] = from_f<T>(acc[r][c] * inv);
+        if (c * 32 + lane < D) dst[c * 32 + lane] = from_f<T>(FP8 ? clamp_finite<T>(acc[r][c] * inv) : acc[r][c] * inv);
       if (p.lse != nullptr && lane == 0) p.lse[(int64_t)h * p.T + row] = lse2 * 0.69314718055994531f;
     } else {
       const int64_t at = ((int64_t)row * p.Hq + h) * p.P + chunk;
@@ -291,7 +291,8 @@ paged_combine_kernel(const Params p, int R, int tk) {
     float a = 0.f;
 #pragma unroll
     for (int w = 0; w < C_WARPS; ++w) a += sm[w][d];
-    dst[d] = from_f<T>(a * inv);
+    a *= inv;
+    dst[d] = from_f<T>(p.v_scale != nullptr ? clamp_finite<T>(a) : a);
   }
   if (p.lse != nullptr && threadIdx.x == 0)
     p.lse[(int64_t)h * p.T + row] =

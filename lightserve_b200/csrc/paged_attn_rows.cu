@@ -556,7 +556,7 @@ paged_rows_kernel(const Params p) {
       for (int w = 0; w < WARPS; ++w) a = fmaf(wt[w], sm_acc[w][r][d], a);
       a *= inv;
       if (chunks == 1)
-        dst[d] = from_f<T>(a);
+        dst[d] = from_f<T>(FP8 ? clamp_finite<T>(a) : a);
       else
         p.part_o[at * D + d] = a;
     }

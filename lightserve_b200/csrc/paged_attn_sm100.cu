@@ -12,9 +12,11 @@
 //    8-row groups, so the box's atoms land as the MMA's descriptors want them; a
 //    box per 64-column half took 13% longer over pages of 16). Pages that do not
 //    exist, or that no row sees, are fetched past the end: zeros.
-//  * e4m3 cache: TMA stages the raw tile, and two converter warpgroups, for K and
-//    V, multiply each row by its power of two in fp32, round to q's type (exact in
-//    bf16, and in fp16 within its range) and write the swizzled tiles.
+//  * e4m3 cache: TMA stages the raw tile, and a converter warpgroup multiplies
+//    each row by its power of two, rounds to q's type (exact in bf16, and in fp16
+//    within its range) and writes the swizzled tiles. (Two converter warpgroups
+//    took the registers of the softmax and were 12% slower; loading the raw
+//    rows into registers instead of staging them, 25%.)
 //  * V rows that no row of the item sees (past the context, between sinks and
 //    window) are zeroed in shared memory, so that what such cells hold never
 //    meets a weight of 0; the tiles that need it are the ends of a span.
@@ -22,7 +24,7 @@
 //    token r / G, head r % G.
 //
 // Warps: 0 loads (Q; K, V of a 16-bit cache), 1 issues MMAs and owns TMEM,
-// 4-7 and 8-11 softmax of query tile 0 and 1; e4m3: 12-15 convert K, 16-19 V.
+// 4-7 and 8-11 softmax of query tile 0 and 1, 12-15 convert (e4m3 only).
 // TMEM: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512) columns. Every
 // mbarrier wait is bounded; on a timeout the error word is set, the role ends,
 // TMEM is freed and the CTA exits.
@@ -159,7 +161,7 @@ __device__ __forceinline__ bool make_item(const Params& p, Item& w) {
 }
 
 template <int D, int FMT, bool FP8>
-__global__ void __launch_bounds__(FP8 ? 640 : 384, 1)
+__global__ void __launch_bounds__(FP8 ? 512 : 384, 1)
 paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                    const __grid_constant__ CUtensorMap tv, const Params p, const int box_log2) {
   using L = Smem<D, FP8>;
@@ -245,7 +247,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   };
 
   // Register split, 384 threads x 168 at launch: 128 x 96 + 256 x 200 = 63,488
-  // of 64,512. e4m3: 640 x 96 at launch: 128 x 48 + 256 x 136 + 256 x 80 = 61,440.
+  // of 64,512. e4m3: 512 x 128 at launch: 128 x (48 + 80) + 256 x 192 = 65,536.
   if (warp == 0) {
     // ------------------------------------------------------------- loads --
     reg_dealloc<FP8 ? 48 : 96>();
@@ -405,7 +407,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     reg_dealloc<FP8 ? 48 : 96>();  // idle members of the first warpgroup
   } else if (warp < 12) {
     // ----------------------------------------------------------- softmax --
-    reg_alloc<FP8 ? 136 : 200>();
+    reg_alloc<FP8 ? 192 : 200>();
     const int t = (warp >> 2) - 1;
     const int row = threadIdx.x - 128 * (t + 1);  // TMEM lane
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -449,39 +451,15 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         for (int cc = 0; cc < 32; ++cc)
           if (!((bits[i] >> cc) & 1)) x[cc] = __float_as_uint(-INFINITY);
       };
-      // 16-bit cache: all 128 scores stay in registers. e4m3: the converter
-      // warpgroups leave room for 64; columns [64, 128) are read once for the
-      // maximum and again after the first half's exponentials.
-      constexpr int HELD = FP8 ? 2 : 4;
-      uint32_t sr[HELD][32];
-      float mx;
-      if constexpr (FP8) {
-        fetch(2, sr[0]);
-        fetch(3, sr[1]);
-        tmem_ld_wait();
-        if (!whole) {
-          hide(2, sr[0]);
-          hide(3, sr[1]);
-        }
-        mx = row_max(sr);
-        fetch(0, sr[0]);
-        fetch(1, sr[1]);
-        tmem_ld_wait();
-        if (!whole) {
-          hide(0, sr[0]);
-          hide(1, sr[1]);
-        }
-        mx = fmaxf(mx, row_max(sr));
-      } else {
+      uint32_t sr[4][32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) fetch(i, sr[i]);
-        tmem_ld_wait();
-        if (!whole) {
+      for (int i = 0; i < 4; ++i) fetch(i, sr[i]);
+      tmem_ld_wait();
+      if (!whole) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) hide(i, sr[i]);
-        }
-        mx = row_max(sr);
+        for (int i = 0; i < 4; ++i) hide(i, sr[i]);
       }
+      const float mx = row_max(sr);
       const float m_new = fmaxf(m, mx * sl2);
       float alpha = 1.f;
       const bool rescale = m_new > m + RESCALE_THRESHOLD;
@@ -507,22 +485,8 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t pk[32];
-        if constexpr (FP8) {
-          if (h == 1) {
-            fetch(2, sr[0]);
-            fetch(3, sr[1]);
-            tmem_ld_wait();
-            if (!whole) {
-              hide(2, sr[0]);
-              hide(3, sr[1]);
-            }
-          }
-          weigh(sr[0], pk);
-          weigh(sr[1], pk + 16);
-        } else {
-          weigh(sr[2 * h], pk);
-          weigh(sr[2 * h + 1], pk + 16);
-        }
+        weigh(sr[2 * h], pk);
+        weigh(sr[2 * h + 1], pk + 16);
         tmem_st32(lane_addr + t * 128 + 32 * h, pk);
         // O is rescaled before the first half's PV accumulates into it; PV_t(j-1)
         // has completed: s_full(j) follows it in issue order.
@@ -605,29 +569,34 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       constexpr int CPR = D / 16;           // 16-byte pieces of a cached row
       constexpr int RPP = 128 / CPR;        // rows per pass of the 128 threads
       constexpr int PASSES = BN / RPP;
-      const bool is_v = warp >= 16;         // 12-15 convert K, 16-19 V
       const int tid = threadIdx.x & 127, c = tid % CPR, r0 = tid / CPR;
-      // A thread's rows r0, r0 + RPP, ... of the tile, 16 bytes of each. Rows that
-      // no row of the item sees become zeros (missing pages arrived as such).
-      auto store = [&](int i, const uint4& raw16, int scale, uint8_t* tile) {
+      auto store = [&](int i, const uint4& raw16, int scale, bool plain, uint8_t* tile) {
         const int kc = c / 4, row = r0 + i * RPP;
-        const float f = e8m0_to_float(scale);
         const uint32_t words[4] = {raw16.x, raw16.y, raw16.z, raw16.w};
         uint32_t o[8];
+        if (FMT == 0 && plain) {  // the scale is an fp16 and no product leaves fp16's range
+          const __half2 f = __half2half2(__float2half_rn(e8m0_to_float(scale)));
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
+          for (int i2 = 0; i2 < 8; ++i2) {
+            const uint32_t z = cvt_e4m3x2_f16x2((uint16_t)(words[i2 / 2] >> (16 * (i2 & 1))));
+            const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&z), f);
+            o[i2] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+        } else {
+          const float f = e8m0_to_float(scale);
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          for (int i2 = 0; i2 < 8; ++i2) {
             const float2 y = __fmul2_rn(
-                f16x2_to_float2(cvt_e4m3x2_f16x2((uint16_t)(words[q4] >> (16 * e)))), make_float2(f, f));
+                f16x2_to_float2(cvt_e4m3x2_f16x2((uint16_t)(words[i2 / 2] >> (16 * (i2 & 1))))),
+                make_float2(f, f));
             if constexpr (FMT == 1) {
-              o[2 * q4 + e] = pack_bf16(y.x, y.y);
+              o[i2] = pack_bf16(y.x, y.y);
             } else {  // a value lifted past fp16's range stays at its largest
               const __half2 top = __float2half2_rn(65504.f);
               const uint32_t z = pack_f16(y.x, y.y);
               const __half2 c2 =
                   __hmax2_nan(__hmin2_nan(*reinterpret_cast<const __half2*>(&z), top), __hneg2(top));
-              o[2 * q4 + e] = *reinterpret_cast<const uint32_t*>(&c2);
+              o[i2] = *reinterpret_cast<const uint32_t*>(&c2);
             }
           }
         }
@@ -638,37 +607,52 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         *reinterpret_cast<uint4*>(base + (((piece + first) ^ (row & 7)) << 4)) = first ? hi : lo;
         *reinterpret_cast<uint4*>(base + (((piece + 1 - first) ^ (row & 7)) << 4)) = first ? lo : hi;
       };
-      uint8_t* tiles = is_v ? sV : sK;
-      uint64_t* full = is_v ? v_full : k_full;
-      uint64_t* empty = is_v ? v_empty : k_empty;
-      const uint8_t* raw = smem + L::RAW_OFF + is_v * L::RAW;
-      const uint8_t* scales = smem + L::SCALE_OFF + is_v * BN;
-      for (int j = 0; j < w.nkv; ++j) {
+      bool ok = true;
+      for (int j = 0; ok && j < w.nkv; ++j) {
         const int s = j % NS, key0 = key0_of(j);
-        if (!mbar_wait_warp(&raw_full[is_v], j & 1, 0x531)) break;
-        uint4 x[PASSES];
-        int e[PASSES];
+        const bool clean = all_seen_by_some(key0, BN);
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint8_t* raw = smem + L::RAW_OFF + kv * L::RAW;
+          const uint8_t* scales = smem + L::SCALE_OFF + kv * BN;
+          uint8_t* tile = smem + (kv ? L::V_OFF : L::K_OFF) + s * L::TILE;
+          if (!mbar_wait_warp(&raw_full[kv], j & 1, 0x531)) { ok = false; break; }
+          uint4 x[PASSES];
+          int e[PASSES];
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          x[i] = *reinterpret_cast<const uint4*>(raw + (r0 + i * RPP) * D + c * 16);
-          e[i] = scales[r0 + i * RPP];
+          for (int i = 0; i < PASSES; ++i) {
+            x[i] = *reinterpret_cast<const uint4*>(raw + (r0 + i * RPP) * D + c * 16);
+            e[i] = scales[r0 + i * RPP];
+          }
+          if (!clean) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i)
+              if (!seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key0 + r0 + i * RPP)) {
+                x[i] = make_uint4(0u, 0u, 0u, 0u);
+                e[i] = 127;
+              }
+          }
+          if (j >= NS && !mbar_wait_warp(kv ? &v_empty[s] : &k_empty[s], ((j / NS) - 1) & 1, 0x532)) {
+            ok = false;
+            break;
+          }
+          // fp16: every scale between 2^-24 and 2^7 (448 2^7 is below 65504).
+          bool plain = true;
+#pragma unroll
+          for (int i = 0; i < PASSES; ++i) plain = plain && e[i] >= 103 && e[i] <= 134;
+          if (FMT == 0) plain = __all_sync(0xffffffffu, plain);
+#pragma unroll
+          for (int i = 0; i < PASSES; ++i) store(i, x[i], e[i], plain, tile);
+          fence_async_shared();
+          __syncwarp();
+          // The raw tile is released once its values have been used: an arrival does
+          // not wait for shared-memory loads still under way, and the next tile's
+          // copy could overtake them.
+          if (lane == 0) {
+            mbar_arrive(kv ? &v_full[s] : &k_full[s]);
+            mbar_arrive(&raw_empty[kv]);
+          }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&raw_empty[is_v]);  // the next tile may come
-        if (!all_seen_by_some(key0, BN)) {
-#pragma unroll
-          for (int i = 0; i < PASSES; ++i)
-            if (!seen_by_any(p, w.pos_lo, w.pos_hi, w.q.ctx, key0 + r0 + i * RPP)) {
-              x[i] = make_uint4(0u, 0u, 0u, 0u);
-              e[i] = 127;
-            }
-        }
-        if (j >= NS && !mbar_wait_warp(&empty[s], ((j / NS) - 1) & 1, 0x532)) break;
-#pragma unroll
-        for (int i = 0; i < PASSES; ++i) store(i, x[i], e[i], tiles + s * L::TILE);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
       }
     }
   }
@@ -767,7 +751,7 @@ static int launch(const Params& p, int dtype, cudaStream_t st) {
   if (int rc_ = limit.ensure(kern, Smem<D, FP8>::ALLOC, "paged_attn smem attribute")) return rc_;
   const int64_t R = (int64_t)(BM / p.G * p.G) * TILES;
   const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)(((int64_t)p.max_q * p.G + R - 1) / R), (unsigned)p.S);
-  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(FP8 ? 640 : 384), Smem<D, FP8>::ALLOC, st, mq, mk, mv, p, box_log2),
+  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(FP8 ? 512 : 384), Smem<D, FP8>::ALLOC, st, mq, mk, mv, p, box_log2),
               "paged_attn");
   return LSB_OK;
 }

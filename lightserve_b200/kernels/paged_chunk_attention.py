@@ -20,28 +20,29 @@ import torch
 from .. import _lib
 
 
-def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, device):
+def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, index):
     """Checks of a 16/32-bit cache of type ``dtype``, or of an e4m3 cache with
-    its scales; returns the cache's C dtype code."""
-    assert k_cache.ndim == 4 and k_cache.shape == v_cache.shape, "caches must be [num_blocks, H, block_size, D]"
+    its scales, on CUDA device ``index`` (-1: CPU); returns the cache's shape and
+    C dtype code."""
+    shape, kind = k_cache.shape, k_cache.dtype
+    assert len(shape) == 4 and shape == v_cache.shape, "caches must be [num_blocks, H, block_size, D]"
     assert k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous"
-    assert k_cache.dtype == v_cache.dtype, f"dtype mismatch: k_cache={k_cache.dtype} v_cache={v_cache.dtype}"
+    assert kind == v_cache.dtype, f"dtype mismatch: k_cache={kind} v_cache={v_cache.dtype}"
     assert (k_scale is None) == (v_scale is None), "k_scale and v_scale go together"
     if k_scale is None:
-        assert k_cache.dtype == dtype, f"q/cache dtypes must match, got {dtype} and {k_cache.dtype}"
+        assert kind == dtype, f"q/cache dtypes must match, got {dtype} and {kind}"
         code = _lib.dtype_code(dtype)
     else:
-        assert k_cache.dtype == torch.float8_e4m3fn, (
-            f"scales go with a float8_e4m3fn cache, got {k_cache.dtype}")
+        assert kind == torch.float8_e4m3fn, f"scales go with a float8_e4m3fn cache, got {kind}"
         assert k_scale.dtype == v_scale.dtype == torch.float8_e8m0fnu, "scales must be float8_e8m0fnu"
-        assert k_scale.shape == v_scale.shape == k_cache.shape[:3], "scales must be [num_blocks, H, block_size]"
+        assert k_scale.shape == v_scale.shape == shape[:3], "scales must be [num_blocks, H, block_size]"
         assert k_scale.is_contiguous() and v_scale.is_contiguous(), "scales must be contiguous"
-        assert k_scale.device == v_scale.device == device, "tensors must be on one device"
+        assert k_scale.get_device() == v_scale.get_device() == index, "tensors must be on one device"
         code = _lib.DTYPE_E4M3
-    assert k_cache.device == v_cache.device == device, "tensors must be on one device"
-    bs = k_cache.shape[2]
+    assert k_cache.get_device() == v_cache.get_device() == index, "tensors must be on one device"
+    bs = shape[2]
     assert bs > 0 and (bs & (bs - 1)) == 0, "block_size must be a power of two"
-    return code
+    return shape, code
 
 
 def _window_args(window, num_sinks):
@@ -66,53 +67,59 @@ def paged_chunk_workspace(q_shape, num_seqs: int, max_seqlen_q: int, num_kv_head
 def _paged_attn(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, max_seqlen_q, window,
                 num_sinks, k_scale, v_scale, scale, out, lse, workspace, impl=_lib.IMPL_AUTO):
     assert q.ndim == 3, f"q must be [T, H, D], got {q.ndim}D"
-    T, Hq, D = q.shape
+    T, Hq, D = shape = q.shape
+    dtype, index, max_q = q.dtype, q.get_device(), int(max_seqlen_q)
     w, sinks = _window_args(window, num_sinks)
-    kv_code = _check_cache(k_cache, v_cache, k_scale, v_scale, q.dtype, q.device)
-    nb, Hkv, bs, Dc = k_cache.shape
+    (nb, Hkv, bs, Dc), kv_code = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, index)
     assert Dc == D, f"cache head dim {Dc} does not match q's {D}"
     assert Hkv > 0 and Hq % Hkv == 0, f"{Hq} query heads are no multiple of the cache's {Hkv}"
-    code = _lib.dtype_code(q.dtype)
-    assert q.stride(2) == 1, "q must be contiguous along D"
+    code = _lib.dtype_code(dtype)
+    sq = q.stride()
+    assert sq[2] == 1, "q must be contiguous along D"
     assert block_tables.dtype == torch.int32 and block_tables.ndim == 2 and block_tables.is_contiguous(), (
         "block_tables must be a contiguous int32 [num_seqs, max_blocks]")
     S, max_blocks = block_tables.shape
     assert context_lens.dtype == torch.int32 and context_lens.shape == (S,) and context_lens.is_contiguous(), (
         "context_lens must be a contiguous int32 [num_seqs]")
-    assert block_tables.device == context_lens.device == q.device, "tensors must be on one device"
+    assert block_tables.get_device() == context_lens.get_device() == index, "tensors must be on one device"
     if cu_seqlens_q is not None:
         assert cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.shape == (S + 1,), (
             "cu_seqlens_q must be int32 [num_seqs + 1]")
-        assert cu_seqlens_q.is_contiguous() and cu_seqlens_q.device == q.device
-        assert 0 <= int(max_seqlen_q) <= T, f"max_seqlen_q {max_seqlen_q} outside [0, {T}]"
+        assert cu_seqlens_q.is_contiguous() and cu_seqlens_q.get_device() == index
+        assert 0 <= max_q <= T, f"max_seqlen_q {max_seqlen_q} outside [0, {T}]"
     else:
         assert S == T, f"one row of q per sequence: q has {T}, block_tables {S}"
-    if out is None:
-        out = torch.empty_like(q)
-    assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.stride(2) == 1
     if lse is not None:
         assert lse.shape == (Hq, T) and lse.dtype == torch.float32 and lse.is_contiguous(), (
             "lse must be a contiguous float32 [H, T]")
-        assert lse.device == q.device
-    assert q.is_cuda, "lightserve_b200 kernels need CUDA tensors"
-    if S == 0 or T == 0 or Hq == 0 or D == 0 or int(max_seqlen_q) == 0:
+        assert lse.get_device() == index
+    assert index >= 0, "lightserve_b200 kernels need CUDA tensors"
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        assert out.shape == shape and out.dtype == dtype and out.get_device() == index
+    so = out.stride()
+    assert so[2] == 1, "out must be contiguous along D"
+    if S == 0 or T == 0 or Hq == 0 or D == 0 or max_q == 0:
         return out
     assert max_blocks > 0 and nb > 0, "empty block table or cache"
     lib = _lib.load()
     if workspace is None:
-        workspace = paged_chunk_workspace(q.shape, S, int(max_seqlen_q), Hkv, max_blocks, bs, q.device,
-                                          window, num_sinks)
-    assert workspace.device == q.device and workspace.is_contiguous()
+        ws_bytes = lib.lsb_paged_attn_workspace_size(S, T, max_q, Hq, Hkv, D, max_blocks, bs, w, sinks)
+        if ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    else:
+        assert workspace.get_device() == index and workspace.is_contiguous()
+        ws_bytes = workspace.numel() * workspace.element_size()
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    with _lib.device_guard(q.device):
+    device = q.device
+    with _lib.device_guard(device):
         rc = lib.lsb_paged_attn(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(k_scale), _lib.ptr(v_scale),
             block_tables.data_ptr(), context_lens.data_ptr(), _lib.ptr(cu_seqlens_q), out.data_ptr(),
-            _lib.ptr(lse), S, T, int(max_seqlen_q), Hq, Hkv, D, max_blocks, bs, nb,
-            q.stride(0), q.stride(1), out.stride(0), out.stride(1), w, sinks, float(scale), code, kv_code,
-            impl, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-            _lib.stream_ptr(q.device),
+            _lib.ptr(lse), S, T, max_q, Hq, Hkv, D, max_blocks, bs, nb, sq[0], sq[1], so[0], so[1], w, sinks,
+            scale, code, kv_code, impl, _lib.ptr(workspace), ws_bytes, _lib.stream_ptr(device),
         )
     _lib.check(rc, "lsb_paged_attn")
     return out

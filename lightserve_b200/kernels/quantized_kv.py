@@ -32,10 +32,10 @@ def quantized_kv_cache(num_blocks: int, num_heads: int, block_size: int, head_di
     return (*rows, *scales)
 
 
-def _check_slots(slot_mapping, T, device):
+def _check_slots(slot_mapping, T, index):
     assert slot_mapping.dtype == torch.int64 and slot_mapping.shape == (T,) and slot_mapping.is_contiguous(), (
         "slot_mapping must be a contiguous int64 [T]")
-    assert slot_mapping.device == device, "tensors must be on one device"
+    assert slot_mapping.get_device() == index, "tensors must be on one device"
 
 
 def quantize_kv_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -44,26 +44,28 @@ def quantize_kv_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     fp32/bf16/fp16) go to slot ``slot_mapping[t]`` (``block_id * block_size +
     offset``; slots outside the cache, such as -1, are skipped). The slots of one
     call must differ: two tokens in one slot leave it with bytes of either."""
-    assert k.ndim == 3 and k.shape == v.shape, f"k/v must be [T, H, D], got {tuple(k.shape)}/{tuple(v.shape)}"
-    T, H, D = k.shape
-    assert k.dtype == v.dtype, f"dtype mismatch: k={k.dtype} v={v.dtype}"
+    shape, dtype, index = k.shape, k.dtype, k.get_device()
+    assert len(shape) == 3 and shape == v.shape, f"k/v must be [T, H, D], got {tuple(shape)}/{tuple(v.shape)}"
+    T, H, D = shape
+    assert dtype == v.dtype, f"dtype mismatch: k={dtype} v={v.dtype}"
     assert k_scale is not None and v_scale is not None, "a quantised cache needs its scales"
-    _check_cache(k_cache, v_cache, k_scale, v_scale, k.dtype, k.device)
-    nb, Hc, bs, Dc = k_cache.shape
-    assert (Hc, Dc) == (H, D), f"cache heads/dim {(Hc, Dc)} do not match k {(H, D)}"
-    code = _lib.dtype_code(k.dtype)
-    assert v.device == k.device, "tensors must be on one device"
-    assert k.stride(2) == 1 and v.stride(2) == 1, "k/v must be contiguous along D"
-    _check_slots(slot_mapping, T, k.device)
-    assert k.is_cuda, "lightserve_b200 kernels need CUDA tensors"
+    (nb, Hc, bs, Dc), _ = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, index)
+    assert Hc == H and Dc == D, f"cache heads/dim {(Hc, Dc)} do not match k {(H, D)}"
+    code = _lib.dtype_code(dtype)
+    assert v.get_device() == index, "tensors must be on one device"
+    sk, sv = k.stride(), v.stride()
+    assert sk[2] == 1 and sv[2] == 1, "k/v must be contiguous along D"
+    _check_slots(slot_mapping, T, index)
+    assert index >= 0, "lightserve_b200 kernels need CUDA tensors"
     if T == 0 or H == 0 or D == 0:
         return
-    lib = _lib.load()
-    with _lib.device_guard(k.device):
+    assert nb > 0, "empty cache"
+    lib, device = _lib.load(), k.device
+    with _lib.device_guard(device):
         rc = lib.lsb_kv_quantize(
             k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), slot_mapping.data_ptr(), T, H, D, nb, bs, k.stride(0), k.stride(1),
-            v.stride(0), v.stride(1), code, _lib.stream_ptr(k.device),
+            v_scale.data_ptr(), slot_mapping.data_ptr(), T, H, D, nb, bs, sk[0], sk[1], sv[0], sv[1], code,
+            _lib.stream_ptr(device),
         )
     _lib.check(rc, "lsb_kv_quantize")
 
@@ -75,32 +77,33 @@ def dequantize_kv_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: t
     (fp32/bf16/fp16), written into ``k_out``/``v_out`` when given. Slots outside
     the cache give zeros; a slot may be read more than once."""
     assert k_scale is not None and v_scale is not None, "a quantised cache needs its scales"
-    code = _lib.dtype_code(dtype)
-    _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, k_cache.device)
-    nb, H, bs, D = k_cache.shape
+    code, index = _lib.dtype_code(dtype), k_cache.get_device()
+    (nb, H, bs, D), _ = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, index)
     assert slot_mapping.ndim == 1, "slot_mapping must be a contiguous int64 [T]"
     T = slot_mapping.shape[0]
-    _check_slots(slot_mapping, T, k_cache.device)
-    outs = []
+    _check_slots(slot_mapping, T, index)
     for o in (k_out, v_out):
-        if o is None:
-            o = torch.empty(T, H, D, dtype=dtype, device=k_cache.device)
-        assert o.shape == (T, H, D) and o.dtype == dtype and o.device == k_cache.device and o.is_contiguous(), (
+        assert o is None or (o.shape == (T, H, D) and o.dtype == dtype and o.get_device() == index
+                             and o.is_contiguous()), (
             f"outputs must be contiguous {dtype} [T, H, D] on the cache's device")
-        outs.append(o)
-    assert k_cache.is_cuda, "lightserve_b200 kernels need CUDA tensors"
+    assert index >= 0, "lightserve_b200 kernels need CUDA tensors"
+    device = k_cache.device
+    if k_out is None:
+        k_out = torch.empty(T, H, D, dtype=dtype, device=device)
+    if v_out is None:
+        v_out = torch.empty(T, H, D, dtype=dtype, device=device)
     if T == 0 or H == 0 or D == 0:
-        return tuple(outs)
+        return k_out, v_out
     assert nb > 0, "empty cache"
     lib = _lib.load()
-    with _lib.device_guard(k_cache.device):
+    with _lib.device_guard(device):
         rc = lib.lsb_kv_dequantize(
             k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            slot_mapping.data_ptr(), outs[0].data_ptr(), outs[1].data_ptr(), T, H, D, nb, bs, code,
-            _lib.stream_ptr(k_cache.device),
+            slot_mapping.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), T, H, D, nb, bs, code,
+            _lib.stream_ptr(device),
         )
     _lib.check(rc, "lsb_kv_dequantize")
-    return tuple(outs)
+    return k_out, v_out
 
 
 def rope_quantize_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -122,47 +125,50 @@ def rope_quantize_kv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
     roundings of ``rope_kv_write``; ``context_lens`` (int32 ``[T]``) receives
     positions + 1. A position outside the tables gives NaN rows in ``q_out`` and
     ``k_out``, context length 0 and no cache write. Returns ``q_out``."""
-    assert qkv.ndim == 4 and qkv.shape[1] == 3 and qkv.stride(3) == 1, "qkv must be [T, 3, H, D]"
-    T, _, H, D = qkv.shape
-    dev = qkv.device
+    shape, sx, dtype, index = qkv.shape, qkv.stride(), qkv.dtype, qkv.get_device()
+    assert len(shape) == 4 and shape[1] == 3 and sx[3] == 1, "qkv must be [T, 3, H, D]"
+    T, _, H, D = shape
     assert D % 2 == 0, f"head dim {D} must be even"
-    code = _lib.dtype_code(qkv.dtype)
+    code = _lib.dtype_code(dtype)
     assert k_scale is not None and v_scale is not None, "a quantised cache needs its scales"
-    _check_cache(k_cache, v_cache, k_scale, v_scale, qkv.dtype, dev)
-    nb, Hc, bs, Dc = k_cache.shape
-    assert (Hc, Dc) == (H, D), f"cache heads/dim {(Hc, Dc)} do not match qkv {(H, D)}"
-    assert cos.ndim == 2 and cos.shape == sin.shape and cos.shape[1] == D and cos.stride() == sin.stride(), (
+    (nb, Hc, bs, Dc), _ = _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, index)
+    assert Hc == H and Dc == D, f"cache heads/dim {(Hc, Dc)} do not match qkv {(H, D)}"
+    table, st = cos.shape, cos.stride()
+    assert len(table) == 2 and table == sin.shape and table[1] == D and st == sin.stride(), (
         "cos and sin must be [max_pos, D] tables of one layout")
-    assert cos.stride(1) == 1 and cos.shape[0] > 0
-    assert qkv.dtype == cos.dtype == sin.dtype == q_out.dtype, "qkv, tables and q_out must share a dtype"
+    assert st[1] == 1 and table[0] > 0
+    assert dtype == cos.dtype == sin.dtype == q_out.dtype, "qkv, tables and q_out must share a dtype"
     assert q_out.shape == (T, H, D) and q_out.is_contiguous()
     if k_out is not None:
-        assert k_out.shape == (T, H, D) and k_out.is_contiguous() and k_out.dtype == qkv.dtype
-        assert k_out.device == dev
+        assert k_out.shape == (T, H, D) and k_out.is_contiguous() and k_out.dtype == dtype
+        assert k_out.get_device() == index
     assert positions.dtype == torch.int64 and positions.shape == (T,) and positions.is_contiguous(), (
         "positions must be a contiguous int64 [T]")
-    assert cos.device == sin.device == q_out.device == positions.device == dev, "tensors must be on one device"
+    assert cos.get_device() == sin.get_device() == q_out.get_device() == positions.get_device() == index, (
+        "tensors must be on one device")
     assert (slot_mapping is None) != (block_tables is None), "give slot_mapping or block_tables, not both"
+    max_blocks = 0
     if slot_mapping is not None:
-        _check_slots(slot_mapping, T, dev)
+        _check_slots(slot_mapping, T, index)
     else:
         assert block_tables.dtype == torch.int32 and block_tables.ndim == 2 and block_tables.shape[0] == T, (
             "block_tables must be int32 [T, max_blocks]")
-        assert block_tables.is_contiguous() and block_tables.shape[1] > 0 and block_tables.device == dev
+        max_blocks = block_tables.shape[1]
+        assert block_tables.is_contiguous() and max_blocks > 0 and block_tables.get_device() == index
     if context_lens is not None:
         assert context_lens.dtype == torch.int32 and context_lens.shape == (T,) and context_lens.is_contiguous()
-        assert context_lens.device == dev
-    assert qkv.is_cuda, "lightserve_b200 kernels need CUDA tensors"
+        assert context_lens.get_device() == index
+    assert index >= 0, "lightserve_b200 kernels need CUDA tensors"
     if T == 0 or H == 0 or D == 0:
         return q_out
-    lib = _lib.load()
-    with _lib.device_guard(dev):
+    assert nb > 0, "empty cache"
+    lib, device = _lib.load(), qkv.device
+    with _lib.device_guard(device):
         rc = lib.lsb_rope_kv_quantize(
-            qkv.data_ptr(), qkv.stride(0), qkv.stride(1), qkv.stride(2), cos.data_ptr(), sin.data_ptr(),
-            cos.stride(0), cos.shape[0], positions.data_ptr(), _lib.ptr(slot_mapping),
-            _lib.ptr(block_tables), 0 if block_tables is None else block_tables.shape[1], q_out.data_ptr(),
-            _lib.ptr(k_out), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), _lib.ptr(context_lens), T, H, D, nb, bs, code, _lib.stream_ptr(dev),
+            qkv.data_ptr(), sx[0], sx[1], sx[2], cos.data_ptr(), sin.data_ptr(), st[0], table[0],
+            positions.data_ptr(), _lib.ptr(slot_mapping), _lib.ptr(block_tables), max_blocks, q_out.data_ptr(),
+            _lib.ptr(k_out), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            _lib.ptr(context_lens), T, H, D, nb, bs, code, _lib.stream_ptr(device),
         )
     _lib.check(rc, "lsb_rope_kv_quantize")
     return q_out

@@ -214,6 +214,28 @@ def test_unequal_scales(new, D):
     _check(b)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("impl", IMPLS)
+@pytest.mark.parametrize("new", [1, 3, 70])
+def test_quantised_values_at_the_ends_of_the_range(new, impl, dtype):
+    """V rows at fp16's largest value (which e4m3 rounds past it; 2^100 in the types whose sums an fp32
+    accumulator must hold) and at the type's smallest: outputs stay finite."""
+    _skip_if_not_served(impl, dtype)
+    b = R.build([new, 90 + new], [new, new], 2, 1, 64, 16, dtype, seed=43)
+    g = torch.Generator().manual_seed(44)
+    top, low = 65504.0 if dtype == F16 else 2.0 ** 100, torch.finfo(dtype).smallest_normal / 8
+    size = torch.tensor([top, -top, low, 1.0], dtype=torch.float64)
+    v = size[torch.randint(0, 4, b["v_cache"].shape[:3], generator=g)][..., None] * torch.ones(64, dtype=torch.float64)
+    (kq, ks), (vq, vs) = (R.quantise(x) for x in (torch.randn(*v.shape, generator=g).to(dtype), v.to(dtype)))
+    b |= {"k_cache": kq.float().to(torch.float8_e4m3fn), "v_cache": vq.float().to(torch.float8_e4m3fn),
+          "k_scale": ks.float().to(torch.float8_e8m0fnu), "v_scale": vs.float().to(torch.float8_e8m0fnu)}
+    out = _run(b, impl=IMPLS[impl])
+    o, tol, _, _ = _want(b)
+    assert bool(out.isfinite().all())
+    # fp16's stored value is above its largest, where the result is held
+    R.check(out, o.clamp(-top, top), tol + (o.abs() - top).clamp(min=0))
+
+
 def test_scale_argument():
     b = R.build([200, 60], [70, 1], 2, 1, 64, 16, F16, seed=13)
     for scale in (0.0, 0.5, -0.3):
@@ -283,11 +305,14 @@ def test_whole_prompts_match_packed_prefill():
 
 @pytest.mark.parametrize("quantised", [False, True])
 @pytest.mark.parametrize("new", [[1, 1, 1], [4, 3, 2], [150, 1, 260]])
-def test_same_inputs_same_bits(new, quantised):
-    b = R.build([1500, 64, 800], new, 2, 2, 128, 16, BF16, quantised=quantised, seed=18)
-    first = _run(b, 400, 4)
-    for _ in range(3):
-        assert torch.equal(first, _run(b, 400, 4))
+@pytest.mark.parametrize("D,G", [(128, 2), (64, 8)])
+def test_same_inputs_same_bits(D, G, new, quantised):
+    b = R.build([1500, 64, 800], new, 2, G, D, 16, BF16, quantised=quantised, seed=18)
+    c = _cuda(b)
+    outs = [paged_chunk_attention(c["q"], c["k_cache"], c["v_cache"], c["block_tables"], c["context_lens"], c["cu"],
+                                  b["most"], window=400, num_sinks=4, k_scale=c["k_scale"], v_scale=c["v_scale"])
+            for _ in range(20)]
+    assert all(torch.equal(outs[0], o) for o in outs)
 
 
 def test_two_calls_on_two_streams():
