@@ -375,30 +375,35 @@ rope_quantize_vec_kernel(const T* __restrict__ qkv, const T* __restrict__ cos_t,
                          const T* __restrict__ sin_t, const RopeArgs a, T* __restrict__ q_out,
                          T* __restrict__ k_out, uint8_t* __restrict__ k_cache,
                          uint8_t* __restrict__ v_cache, uint8_t* __restrict__ k_scale,
-                         uint8_t* __restrict__ v_scale, const CellOf cell_of, uint32_t rows,
-                         const FastDiv heads) {
+                         uint8_t* __restrict__ v_scale, const CellOf cell_of, uint32_t units,
+                         const FastDiv head_groups) {
   allow_dependents();
   wait_prerequisites();
   constexpr int VEC = 16 / sizeof(T);
   constexpr int LPR = D / VEC;
   static_assert(LPR >= 2 && LPR <= 32, "a row and its rotary partner live in one warp");
   const uint64_t g = (uint64_t)blockIdx.x * THREADS + threadIdx.x;
-  const bool in = g / LPR < rows;
-  const uint32_t row = in ? (uint32_t)(g / LPR) : rows - 1;
+  const bool in = g / LPR < units;
   const int c = (int)(g % LPR);
-  uint32_t t, h;
-  heads.split(row, t, h);
-  const T* x = qkv + t * a.s_s + h * a.s_h + c * VEC;
-  const Vec16<T> qx = ld_vec16_stream(x), kx = ld_vec16_stream(x + a.s_part),
-                 vx = ld_vec16_stream(x + 2 * a.s_part);
+  uint32_t t, hg;
+  head_groups.split(in ? (uint32_t)(g / LPR) : units - 1, t, hg);
+  const uint32_t h0 = hg * QPT, H = cell_of.H;
+  Vec16<T> qx[QPT], kx[QPT], vx[QPT];
+#pragma unroll
+  for (int i = 0; i < QPT; ++i) {
+    const T* x = qkv + t * a.s_s + min(h0 + i, H - 1) * a.s_h + c * VEC;
+    qx[i] = ld_vec16_stream(x);
+    kx[i] = ld_vec16_stream(x + a.s_part);
+    vx[i] = ld_vec16_stream(x + 2 * a.s_part);
+  }
   const int64_t pos = a.positions[t];
   // A position outside the table has no angle: q (and k_out) become NaN and
   // nothing is cached.
   const bool known = pos >= 0 && pos < a.max_pos;
   const Vec16<T> cx = ld_vec16(cos_t + (known ? pos : 0) * a.s_pos + c * VEC);
   const Vec16<T> sx = ld_vec16(sin_t + (known ? pos : 0) * a.s_pos + c * VEC);
-  const int64_t cell = in && known ? cell_of(t, h) : -1;
-  if (in && h == 0 && c == 0 && a.context_lens != nullptr)
+  const int64_t cell = in && known ? cell_of(t, h0) : -1;
+  if (in && h0 == 0 && c == 0 && a.context_lens != nullptr)
     a.context_lens[t] = known ? (int32_t)(pos + 1) : 0;
   Vec16<T> sn;  // the first half takes -x2, the second x1
   {
@@ -419,13 +424,19 @@ rope_quantize_vec_kernel(const T* __restrict__ qkv, const T* __restrict__ cos_t,
       for (int e = 0; e < VEC; ++e) out.v[e] = from_f<T>(__int_as_float(0x7fc00000));
     }
   };
-  Vec16<T> o;
-  turn(qx, o);
-  if (in) st_vec16(q_out + (int64_t)row * D + c * VEC, o);
-  turn(kx, o);
-  if (in && k_out != nullptr) st_vec16(k_out + (int64_t)row * D + c * VEC, o);
-  store_row<LPR>(o, cell, c, D, k_cache, k_scale);
-  store_row<LPR>(vx, cell, c, D, v_cache, v_scale);
+#pragma unroll
+  for (int i = 0; i < QPT; ++i) {
+    const bool here = in && h0 + i < H;
+    const int64_t o = ((int64_t)t * H + h0 + i) * D + c * VEC;
+    const int64_t at = cell >= 0 && here ? cell + (int64_t)i * cell_of.bs : -1;
+    Vec16<T> r;
+    turn(qx[i], r);
+    if (here) st_vec16(q_out + o, r);
+    turn(kx[i], r);
+    if (here && k_out != nullptr) st_vec16(k_out + o, r);
+    store_row<LPR>(r, at, c, D, k_cache, k_scale);
+    store_row<LPR>(vx[i], at, c, D, v_cache, v_scale);
+  }
 }
 
 template <typename T>
@@ -633,13 +644,14 @@ extern "C" int lsb_rope_kv_quantize(const void* qkv, int64_t s_s, int64_t s_part
                      strides16(sizeof(Tt), {s_s, s_part, s_h, s_pos});
     const int rc = vec ? with_dim<Tt>(D, [&](auto dim) -> int {
       constexpr int DD = decltype(dim)::value;
-      const unsigned blocks = blocks_for(rows, DD * (int)sizeof(Tt) / 16);
+      const uint32_t groups = (uint32_t)((H + QPT - 1) / QPT), units = (uint32_t)T * groups;
+      const unsigned blocks = blocks_for(units, DD * (int)sizeof(Tt) / 16);
       LSB_CHECK_ARG(blocks > 0, "rope_kv_quantize: too many rows");
       LSB_CUDA_OK(lsb::launch_kernel(rope_quantize_vec_kernel<Tt, DD>, dim3(blocks), dim3(THREADS),
                                      0, st, (const Tt*)qkv, (const Tt*)cos_table,
                                      (const Tt*)sin_table, args, (Tt*)q_out, (Tt*)k_out,
                                      (uint8_t*)k_cache, (uint8_t*)v_cache, (uint8_t*)k_scale,
-                                     (uint8_t*)v_scale, cell_of, rows, heads),
+                                     (uint8_t*)v_scale, cell_of, units, FastDiv(groups)),
                   "rope_kv_quantize");
       return LSB_OK;
     }) : -1;
