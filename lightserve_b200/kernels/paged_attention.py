@@ -52,7 +52,7 @@ def paged_decode_workspace(q_shape, max_blocks_per_seq: int, block_size: int, de
     keyword arguments say how ``paged_decode_attention`` will be called:
     the cache's heads where they are fewer than q's, an e4m3 cache, a window."""
     S, H, D = q_shape
-    if quantized or window is not None or num_kv_heads not in (None, H):
+    if quantized or window is not None or num_sinks or num_kv_heads not in (None, H):
         return paged_chunk_workspace(q_shape, S, 1, num_kv_heads or H, max_blocks_per_seq, block_size,
                                      device, window, num_sinks)
     nbytes = _lib.load().lsb_paged_decode_workspace_size(S, H, D, max_blocks_per_seq, block_size)

@@ -27,6 +27,13 @@ cache through each token's slot, ``flash_attention_varlen`` attends within
 each prompt); other models prefill one request at a time through
 ``llama_forward``.
 
+Options beyond lightserve's decode, off by default: an e4m3 cache
+(``PagedKVCache(quantized=True)``), a sliding window with a few first tokens that
+stay visible (``window``, ``num_sinks``), and prompts prefilled in chunks of at
+most ``prefill_chunk_tokens`` (which bounds the activations of a long prompt).
+With any of them the prefill writes each chunk's K/V into the cache and attends
+over the cache (``paged_chunk_attention``), for every dtype.
+
 Block reservation: at admission the runner asks the block manager for every
 block the request will need over ``max_new_tokens`` (``allocate`` for the
 prompt, then the same ``append_slot`` sequence the scheduler would issue one
@@ -48,21 +55,33 @@ from ..kernels.linear import linear, pack_linear_weight
 from ..kernels.sampling import greedy_next
 from ..kernels.paged_attention import (paged_decode_attention, paged_decode_workspace,
                                         rope_kv_write, rope_kv_write_slots, write_kv_cache)
+from ..kernels.paged_chunk_attention import paged_chunk_attention
+from ..kernels.quantized_kv import quantized_kv_cache, rope_quantize_kv
 from .minimal_llama import LlamaConfig, LlamaWeights, llama_forward, precompute_rope
 
 
 class PagedKVCache:
-    """Per-layer K and V pools of shape [num_blocks, n_heads, block_size, head_dim]."""
+    """Per-layer K and V pools of shape [num_blocks, n_heads, block_size, head_dim]
+    in the model dtype, or (``quantized``) in e4m3 with per-row scales
+    ``k_scale``/``v_scale`` (``quantized_kv_cache``; None otherwise)."""
 
-    def __init__(self, config: LlamaConfig, num_blocks: int, block_size: int = 16, device="cuda"):
+    def __init__(self, config: LlamaConfig, num_blocks: int, block_size: int = 16, device="cuda",
+                 quantized: bool = False):
         shape = (num_blocks, config.n_heads, block_size, config.head_dim)
         self.block_size = block_size
         self.num_blocks = num_blocks
+        self.quantized = quantized
+        if quantized:
+            pools = [quantized_kv_cache(*shape, device=device) for _ in range(config.n_layers)]
+            self.k, self.v, self.k_scale, self.v_scale = (list(t) for t in zip(*pools))
+            return
+        self.k_scale = self.v_scale = [None] * config.n_layers
         self.k = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in range(config.n_layers)]
         self.v = [torch.zeros(shape, dtype=config.dtype, device=device) for _ in range(config.n_layers)]
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in self.k + self.v)
+        return sum(t.numel() * t.element_size()
+                   for t in [*self.k, *self.v, *self.k_scale, *self.v_scale] if t is not None)
 
 
 def slots_for_positions(table, positions, block_size: int):
@@ -87,8 +106,13 @@ class PagedDecoder:
 
     def __init__(self, weights: LlamaWeights, config: LlamaConfig, cache: PagedKVCache,
                  block_manager: BlockManager, max_batch: int, max_blocks_per_seq: int,
-                 device="cuda", use_lsb_linear: bool = False):
+                 device="cuda", use_lsb_linear: bool = False, window: int | None = None,
+                 num_sinks: int = 0, prefill_chunk_tokens: int | None = None):
+        assert prefill_chunk_tokens is None or prefill_chunk_tokens > 0, "prefill_chunk_tokens must be positive"
         self.w, self.cfg, self.cache, self.bm = weights, config, cache, block_manager
+        self.window, self.num_sinks, self.prefill_chunk_tokens = window, num_sinks, prefill_chunk_tokens
+        # Prefill attends over the cache, not over the prompt's own K/V.
+        self.over_cache = cache.quantized or window is not None or prefill_chunk_tokens is not None
         self.device = torch.device(device)
         self.S, self.MB = max_batch, max_blocks_per_seq
         self.fused = [_Fused(torch.cat([l.q_proj, l.k_proj, l.v_proj], dim=1).t().contiguous(),
@@ -119,7 +143,8 @@ class PagedDecoder:
         self.attn_out = torch.empty(S, H, D, dtype=config.dtype, device=dev)
         self.q_rot = torch.empty(S, H, D, dtype=config.dtype, device=dev)
         self.act = torch.empty(S, config.intermediate_size, dtype=config.dtype, device=dev)
-        self.ws = paged_decode_workspace((S, H, D), max_blocks_per_seq, cache.block_size, dev)
+        self.ws = paged_decode_workspace((S, H, D), max_blocks_per_seq, cache.block_size, dev,
+                                         quantized=cache.quantized, window=window, num_sinks=num_sinks)
         self.graph = None
         self.requests: list = []
 
@@ -135,7 +160,8 @@ class PagedDecoder:
         assert len(requests) <= self.S
         bs = self.cache.block_size
         if packed is None:
-            packed = self.packed_prefill_supported()
+            packed = self.over_cache or self.packed_prefill_supported()
+        assert packed or not self.over_cache, "this decoder prefills over the cache only"
         first = []
         tables = []
         for r in requests:
@@ -186,7 +212,7 @@ class PagedDecoder:
         next token (host ints). Packed when supported, else one at a time."""
         if not token_lists:
             return []
-        if self.packed_prefill_supported():
+        if self.over_cache or self.packed_prefill_supported():
             return self.prefill_sequences(token_lists, tables).tolist()
         return [int(self._prefill_one(t, tb)) for t, tb in zip(token_lists, tables)]
 
@@ -198,6 +224,8 @@ class PagedDecoder:
         """One forward over every token of ``token_lists`` (packed along the
         token axis), writing each token's K/V into its cache slot; returns the
         greedy next token of each sequence (int64 [len(token_lists)])."""
+        if self.over_cache:
+            return self._prefill_over_cache(token_lists, tables)
         assert self.packed_prefill_supported()
         cfg, bs, dev = self.cfg, self.cache.block_size, self.device
         H, D, Hd = cfg.n_heads, cfg.head_dim, cfg.hidden_size
@@ -230,6 +258,72 @@ class PagedDecoder:
         final, _ = fused_add_rmsnorm(x[last].contiguous(), residual[last].contiguous(), self.w.norm_weight,
                                      eps=cfg.rms_eps)
         return (final @ self.w.lm_head).argmax(-1)
+
+    def _prefill_over_cache(self, token_lists, tables) -> torch.Tensor:
+        """``prefill_sequences`` in chunks of at most ``prefill_chunk_tokens`` packed
+        tokens (a sequence may span several): each chunk's K/V goes into the
+        cache, then its tokens attend to everything their sequence has cached."""
+        bs, dev = self.cache.block_size, self.device
+        lens = [len(t) for t in token_lists]
+        assert min(lens) > 0, "empty prompt"
+        assert max(lens) <= self.cfg.max_seq_len, "sequence longer than the RoPE table"
+        bt = torch.full((len(tables), self.MB), -1, dtype=torch.int32)
+        for i, tb in enumerate(tables):
+            assert len(tb) <= self.MB, "max_blocks_per_seq too small"
+            bt[i, :len(tb)] = torch.as_tensor(tb, dtype=torch.int32)
+        bt = bt.to(dev)
+        nxt = torch.empty(len(lens), dtype=torch.int64, device=dev)
+        pieces = [(i, 0) for i in range(len(lens))]  # (sequence, first token to do), in order
+        while pieces:
+            room = self.prefill_chunk_tokens or sum(lens)
+            chunk = []
+            while pieces and room > 0:
+                i, a = pieces.pop(0)
+                b = min(lens[i], a + room)
+                chunk.append((i, a, b))
+                room -= b - a
+                if b < lens[i]:
+                    pieces.insert(0, (i, b))
+            sizes = [b - a for _, a, b in chunk]
+            ids = torch.tensor([t for i, a, b in chunk for t in token_lists[i][a:b]], dtype=torch.int64)
+            positions = torch.cat([torch.arange(a, b, dtype=torch.int64) for _, a, b in chunk])
+            slots = torch.cat([slots_for_positions(tables[i], range(a, b), bs) for i, a, b in chunk])
+            cu = torch.tensor([0] + torch.tensor(sizes).cumsum(0).tolist(), dtype=torch.int32)
+            ctx = torch.tensor([b for _, _, b in chunk], dtype=torch.int32)
+            rows = torch.tensor([i for i, _, _ in chunk])
+            ends = [(j, i) for j, (i, _, b) in enumerate(chunk) if b == lens[i]]
+            x, residual = self._chunk_layers(*(t.to(dev) for t in (ids, positions, slots, cu, ctx)),
+                                             bt[rows.to(dev)], max(sizes))
+            if ends:
+                last = (cu[1:][[j for j, _ in ends]] - 1).long().to(dev)
+                final, _ = fused_add_rmsnorm(x[last], residual[last], self.w.norm_weight, eps=self.cfg.rms_eps)
+                nxt[torch.tensor([i for _, i in ends], device=dev)] = (final @ self.w.lm_head).argmax(-1)
+        return nxt
+
+    def _chunk_layers(self, ids, positions, slots, cu, ctx, bt, longest):
+        """Every layer over one chunk; returns the residual stream's (x, residual)."""
+        cfg, c, T = self.cfg, self.cache, ids.shape[0]
+        H, D, Hd = cfg.n_heads, cfg.head_dim, cfg.hidden_size
+        residual = F.embedding(ids, self.w.embed_tokens)
+        x = torch.zeros_like(residual)
+        q_rot = torch.empty(T, H, D, dtype=cfg.dtype, device=self.device)
+        attn = torch.empty_like(q_rot)
+        for li, layer in enumerate(self.w.layers):
+            fz = self.fused[li]
+            normed, residual = fused_add_rmsnorm(x, residual, layer.input_layernorm_weight, eps=cfg.rms_eps)
+            qkv = (normed @ fz.w_qkv_t.t()).view(T, 3, H, D)
+            if c.quantized:
+                rope_quantize_kv(qkv, self.cos, self.sin, positions, q_rot, c.k[li], c.v[li], c.k_scale[li],
+                                 c.v_scale[li], slot_mapping=slots)
+            else:
+                rope_kv_write_slots(qkv, self.cos, self.sin, positions, slots, q_rot, None, c.k[li], c.v[li])
+            paged_chunk_attention(q_rot, c.k[li], c.v[li], bt, ctx, cu, longest, window=self.window,
+                                  num_sinks=self.num_sinks, k_scale=c.k_scale[li], v_scale=c.v_scale[li], out=attn)
+            x = attn.view(T, Hd) @ layer.o_proj
+            normed2, residual = fused_add_rmsnorm(x, residual, layer.post_attention_layernorm_weight,
+                                                  eps=cfg.rms_eps)
+            x = silu_and_mul(normed2 @ fz.w_gu_t.t()) @ layer.down_proj
+        return x, residual
 
     # ------------------------------------------------------- slot decode --
     def decode_slots(self, slots, tokens, positions, tables, use_graph: bool = True) -> list:
@@ -300,10 +394,17 @@ class PagedDecoder:
             qkv = mm(normed, fz.w_qkv_t).view(S, 3, H, D)
             # RoPE at each sequence's position + K/V into its cache slot, fused
             # (also sets context_lens = positions + 1).
-            q = rope_kv_write(qkv, self.cos, self.sin, pos, self.block_tables, self.q_rot,
-                              self.cache.k[li], self.cache.v[li], self.context_lens)
-            attn = paged_decode_attention(q, self.cache.k[li], self.cache.v[li], self.block_tables,
-                                          self.context_lens, out=self.attn_out, workspace=self.ws)
+            c = self.cache
+            if c.quantized:
+                q = rope_quantize_kv(qkv, self.cos, self.sin, pos, self.q_rot, c.k[li], c.v[li], c.k_scale[li],
+                                     c.v_scale[li], block_tables=self.block_tables,
+                                     context_lens=self.context_lens)
+            else:
+                q = rope_kv_write(qkv, self.cos, self.sin, pos, self.block_tables, self.q_rot,
+                                  c.k[li], c.v[li], self.context_lens)
+            attn = paged_decode_attention(q, c.k[li], c.v[li], self.block_tables, self.context_lens,
+                                          out=self.attn_out, workspace=self.ws, window=self.window,
+                                          num_sinks=self.num_sinks, k_scale=c.k_scale[li], v_scale=c.v_scale[li])
             x = mm(attn.view(S, Hd), fz.w_o_t)
             normed2, residual = fused_add_rmsnorm(x, residual, layer.post_attention_layernorm_weight,
                                                   eps=cfg.rms_eps)

@@ -30,7 +30,12 @@ from .paged_decode import PagedDecoder, PagedKVCache
 class ServingEngine:
     def __init__(self, weights: LlamaWeights, config: LlamaConfig, cache_config: CacheConfig,
                  scheduler_config: SchedulerConfig, device="cuda", use_graph: bool = True,
-                 check_every: int = 64):
+                 check_every: int = 64, quantized_kv: bool = False, window: int | None = None,
+                 num_sinks: int = 0, prefill_chunk_tokens: int | None = None):
+        """``quantized_kv``, ``window``, ``num_sinks`` and ``prefill_chunk_tokens`` are the
+        options of ``PagedKVCache`` and ``PagedDecoder`` of those names (the
+        scheduler's policy does not change: an admitted prompt is prefilled in
+        one step, of as many chunks as it takes)."""
         self.cfg = config
         # Every `check_every` steps (and at the end of run()) the device error
         # words are read: a kernel that gave up on a bounded wait raises
@@ -39,11 +44,12 @@ class ServingEngine:
         self._steps = 0
         self.scheduler = Scheduler(cache_config, scheduler_config)
         bs = cache_config.block_size
-        self.cache = PagedKVCache(config, cache_config.num_gpu_blocks, bs, device=device)
+        self.cache = PagedKVCache(config, cache_config.num_gpu_blocks, bs, device=device, quantized=quantized_kv)
         max_blocks = -(-config.max_seq_len // bs)
         self.runner = PagedDecoder(weights, config, self.cache, self.scheduler.block_manager,
                                    max_batch=scheduler_config.max_num_seqs,
-                                   max_blocks_per_seq=max_blocks, device=device)
+                                   max_blocks_per_seq=max_blocks, device=device, window=window,
+                                   num_sinks=num_sinks, prefill_chunk_tokens=prefill_chunk_tokens)
         self.use_graph = use_graph
         self.slot_of: dict = {}
         self._free_slots = list(range(scheduler_config.max_num_seqs - 1, -1, -1))
