@@ -342,8 +342,13 @@ static Plan plan_simt(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t 
   return plan_split(S * Hkv * ((max_q * G + SR - 1) / SR), keys, 4 * 148, 128);
 }
 
-// Pairs up to which the few-rows kernel is taken where it serves the call.
-constexpr int64_t ROWS_MAX_PAIRS = 64;
+// Pairs up to which the few-rows kernel is taken where it serves the call: one
+// of its tiles. Measured with both kernels, bf16: 32 sequences of 512-4096
+// keys, 8 cache heads of 128, 20 pairs: 84 us against the tcgen05 kernel's 105
+// (1000-2000 keys, 16 / 24 / 32 pairs: 60 / 74 / 106 against 62); 16 heads of
+// 64: 24 / 32 pairs 88 / 131 against 98; one sequence of 16000 keys, 8 heads of
+// 128: 16 / 24 / 32 pairs 21.0 / 24 / 33 against 21; e4m3 alike.
+constexpr int64_t ROWS_MAX_PAIRS = 24;
 
 static Plan plan_rows(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t keys) {
   if (max_q * G > ROWS_MAX_PAIRS) return {1 << 30, 1};

@@ -186,6 +186,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::TMEM_SLOT_OFF);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tq);
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
   allow_dependents();
   wait_prerequisites();
   Item w;
@@ -252,7 +257,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     // ------------------------------------------------------------- loads --
     reg_dealloc<FP8 ? 48 : 96>();
     if (lane == 0) {
-      prefetch_tmap(&tq);
       const int tokens = w.R / p.G;
 #pragma unroll
       for (int t = 0; t < TILES; ++t) {
