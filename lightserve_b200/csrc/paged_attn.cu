@@ -460,7 +460,7 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
   const Plan rows_plan = plan_rows(num_seqs, max_seqlen_q, Hkv, p.G, keys);
   const Plan tc_plan = plan_tc(num_seqs, max_seqlen_q, Hkv, p.G, keys);
   p.P = std::max(rows_plan.P, tc_plan.P);  // (the grids' limits)
-  const bool rows_ok = rows_eligible(p, dtype, fp8), tc_ok = tc_eligible(p, dtype, fp8);
+  const bool rows_ok = rows_eligible(p, dtype), tc_ok = tc_eligible(p, dtype, fp8);
   LSB_CHECK_ARG(impl != LSB_IMPL_ROWS || rows_ok,
                 "paged_attn: the few-rows kernel needs bf16/fp16, D in {64,128}, pages of 8 keys or "
                 "more, q strides that are multiples of 4 elements and 16-byte aligned caches");
@@ -496,7 +496,7 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
   if (impl == LSB_IMPL_ROWS) {
     const int rc = launch_rows(p, dtype, fp8, st);
     if (rc != LSB_OK || p.P == 1) return rc;
-    return launch_combine(p, rows_tile(max_seqlen_q * p.G), ROWS_TK, dtype, st);
+    return launch_combine(p, rows_tile(max_seqlen_q * p.G), rows_tk(fp8), dtype, st);
   }
   if (impl == LSB_IMPL_TCGEN05) {
     const int rc = launch_tc(p, dtype, fp8, st);

@@ -133,12 +133,12 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 // paged_attn_rows.cu's key group, and the pairs of its query tile: 8, 16 or 24,
 // the fewest that hold a sequence's (more pairs take several tiles, each of
 // which reads the cache again).
-constexpr int ROWS_TK = 16;
+constexpr int rows_tk(bool kv_fp8) { return kv_fp8 ? 32 : 16; }
 inline int rows_tile(int64_t pairs) { return pairs <= 8 ? 8 : pairs <= 16 ? 16 : 24; }
 constexpr int TC_TK = 128;  // paged_attn_sm100.cu's key tile; a query tile holds (128 / G) G pairs
 bool tc_eligible(const Params& p, int dtype, bool kv_fp8);
 int launch_tc(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
-bool rows_eligible(const Params& p, int dtype, bool kv_fp8);
+bool rows_eligible(const Params& p, int dtype);
 int launch_rows(const Params& p, int dtype, bool kv_fp8, cudaStream_t st);
 
 }  // namespace pa

@@ -20,10 +20,11 @@
 //    8 + 2t and 9 + 2t at dims (8 i + g) EV and interleaves key pairs with byte
 //    permutes; its dims are rows g and 8 + g of the m-tiles in turn.
 //
-// Each warp streams its groups through a ring of its own in shared memory
-// (cp.async, 16 bytes a lane: STAGES groups in flight cost no registers and no
-// barrier beyond the warp's). Rows are stored with their 16-byte pieces permuted
-// (Shape::at) so that both kinds of read touch every bank once.
+// Each warp streams its groups through a ring of its own in shared memory, a TMA
+// box per page, tensor and group issued by one lane (copying 16 bytes a lane
+// with cp.async took a third of all instructions). The boxes' swizzle and the
+// order in which a group's keys are the MMA's rows (sigma) make both kinds of
+// read touch every bank once.
 //
 // e4m3 cache: bytes convert to fp16 in one instruction per pair (exactly; the
 // MMAs run in fp16), unscaled. K's power-of-two scale multiplies the score. V's
@@ -40,6 +41,7 @@
 // relative to each weight, as in the framework's other attention kernels.
 #include "paged_attn.cuh"
 #include "sm100.cuh"
+#include "tma_host.cuh"
 
 #include <type_traits>
 
@@ -48,7 +50,6 @@ namespace pa {
 
 namespace rows {
 
-constexpr int TK = ROWS_TK;  // keys per group
 constexpr int WARPS = 4;
 constexpr float RAISE = 8.f;   // log2: how far a score may exceed the reference maximum
 constexpr float LIFT = 7.f;    // log2: factor on every weight
@@ -90,26 +91,32 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[N], const void* p) {
   }
 }
 
-// 16 bytes (8: scales) from global to shared memory, zeros when !there.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(there ? 16 : 0)
-               : "memory");
+// Key of a half group that is the MMA's row r, such that the rows read by eight
+// consecutive lanes have swizzle patterns that do not collide.
+__device__ __forceinline__ int sigma(int r) { return r ^ ((r & 1) << 2); }
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
 }
-__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(there ? 8 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                            int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
 }
 
 template <bool FP8, int D>
 struct Shape {
   static constexpr int EB = FP8 ? 1 : 2;           // bytes per cached element
+  static constexpr int TK = rows_tk(FP8);          // keys per group
+  static constexpr int NU = TK / 16;               // MMA row blocks of a group
+  static constexpr int GR = TK / 8;                // runs of 8 keys, each within a page
   static constexpr int EK = 16 / EB;               // K elements per lane and load
   static constexpr int NK = D / (4 * EK);          // K loads per key and lane
   static constexpr int EV = FP8 ? D / 8 : 8;       // V elements per lane and load
@@ -118,23 +125,19 @@ struct Shape {
   static constexpr int STEPS = D / 16;             // k steps of S^T
   static constexpr int MT = D / 16;                // m-tiles of O^T
   static constexpr int CPR = D * EB / 16;          // 16-byte pieces of a row: 4, 8 or 16
-  static constexpr int HALF = 8 * CPR;             // pieces of 8 keys
   static constexpr int TILE = TK * CPR * 16;       // bytes of a group's K (and V)
-  // A stage: K, V, and for e4m3 the scales (16 of K, 16 of V).
-  static constexpr int STAGE = 2 * TILE + (FP8 ? 32 : 0);
+  static constexpr int STAGE = 2 * TILE;
   // Groups in flight per warp, sized so that an SM holds about 190 KB of ring.
-  static constexpr int STAGES = FP8 ? 4 : (D == 64 ? 4 : 3);
+  static constexpr int STAGES = FP8 ? (D == 64 ? 3 : 2) : (D == 64 ? 4 : 3);
   static constexpr int ctas(int nh) {
-    return FP8 ? (D == 64 ? 6 - nh : (nh == 3 ? 2 : 3)) : (D == 64 ? 3 : 2);
+    return FP8 ? (D == 64 ? (nh == 1 ? 4 : 3) : (nh == 3 ? 2 : 3)) : (D == 64 ? 3 : 2);
   }
-  // Byte offset of piece c of key k's row in its tile.
+  // Byte offset of 16-byte piece c of key k's row in its tile, as the boxes of
+  // up to 16 rows and their swizzle leave it (256-byte rows come in two halves
+  // of 128).
   static __device__ __forceinline__ int at(int k, int c) {
-    if constexpr (CPR == 4) {  // two rows to a 128-byte line
-      const int line = k >> 1;
-      return (line * 8 + ((((k & 1) << 2) | c) ^ ((line & 3) << 1))) * 16;
-    } else {
-      return (k * CPR + (c ^ ((((k >> 1) & 3) << 1) ^ ((k & 1) << 2)))) * 16;
-    }
+    if constexpr (CPR == 4) return k * 64 + ((c ^ ((k >> 1) & 3)) << 4);
+    return (k >> 4) * (CPR * 256) + (c >> 3) * 2048 + (k & 15) * 128 + (((c & 7) ^ (k & 7)) << 4);
   }
 };
 
@@ -143,18 +146,25 @@ template <bool FP8, int D, int NH>
 constexpr int smem_bytes() {
   const int ring = WARPS * Shape<FP8, D>::STAGES * Shape<FP8, D>::STAGE;
   const int merge = WARPS * 8 * NH * (D + 4 + 3) * 4;
-  return ring > merge ? ring : merge;
+  return (ring > merge ? ring : merge) + 1024;  // slack for 1024-byte alignment
 }
 
 template <typename T, bool FP8, int D, int NH>
 __global__ void __launch_bounds__(WARPS * 32, (Shape<FP8, D>::ctas(NH)))
-paged_rows_kernel(const Params p) {
+paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                  const Params p) {
+  if (threadIdx.x == 0) {
+    sm100::prefetch_tmap(&tk);
+    sm100::prefetch_tmap(&tv);
+  }
   allow_dependents();
   wait_prerequisites();
   using S = Shape<FP8, D>;
   constexpr bool F16 = FP8 || std::is_same<T, __half>::value;  // MMA operand type
-  constexpr int R = 8 * NH;
-  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int R = 8 * NH, TK = S::TK, NU = S::NU;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (sm100::smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t bars[WARPS][S::STAGES];  // a group's boxes have arrived
 
   const int chunk = blockIdx.x % p.P, hk = blockIdx.x / p.P, tile = blockIdx.y, s = blockIdx.z;
   const Seq q = load_seq(p, s);
@@ -173,77 +183,91 @@ paged_rows_kernel(const Params p) {
   const int bs = 1 << p.bs_log2;
 
   // ------------------------------------------------------------- loads ----
-  // Page ids of 16 of this warp's groups from v on, one half group per lane;
-  // -1: no such page.
+  // Page ids of the next BATCH of this warp's groups from v on, one run of 8 keys
+  // per lane; -1: no such page.
+  constexpr int BATCH = 32 / S::GR;
   auto fetch_ids = [&](int v) -> int {
-    const int vv = v + (lane >> 1) * WARPS;
+    const int vv = v + lane / S::GR * WARPS;
     if (vv >= v1) return -1;
-    const int tok = span.tile(vv) * TK + 8 * (lane & 1);
+    const int tok = span.tile(vv) * TK + 8 * (lane % S::GR);
     if (tok >= q.ctx) return -1;
     const int id = bt[tok >> p.bs_log2];
     return id >= 0 && id < p.num_blocks ? id : -1;
   };
-  const uint8_t* kc = static_cast<const uint8_t*>(p.k_cache) + lane * 16;
-  const uint8_t* vc = static_cast<const uint8_t*>(p.v_cache) + lane * 16;
   uint8_t* ring = smem + warp * (S::STAGES * S::STAGE);
-  // Whether every pair sees all 16 keys at tok0 (pages apart).
+  uint64_t* full = bars[warp];
+  if (lane == 0) {
+    for (int i = 0; i < S::STAGES; ++i) sm100::mbar_init(&full[i], 1);
+    sm100::fence_barrier_init();
+  }
+  __syncwarp();
+  // Whether every pair sees all TK keys at tok0 (pages apart).
   auto all_seen = [&](int tok0) -> bool {
     const int last = tok0 + TK - 1;
     return last <= pos_lo && last < q.ctx &&
            (p.window == 0 || pos_hi - tok0 < p.window || last < p.sinks);
   };
-  // Copies the group at keys [tok0, tok0 + 16) into a stage. Missing pages and
-  // V rows that no row of the tile sees arrive as zeros, so what such cells
-  // hold never meets a weight of 0.
-  auto copy_group = [&](int stage, int tok0, int id0, int id1) {
-    const uint32_t dst = sm100::smem_u32(ring + stage * S::STAGE);
-    const bool clean = id0 >= 0 && id1 >= 0 && all_seen(tok0);
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int id = hf == 0 ? id0 : id1;
-      const int64_t cell =
-          ((int64_t)max(id, 0) * p.Hkv + hk) * bs + ((tok0 + 8 * hf) & (bs - 1));
-      const uint8_t* ks = kc + cell * (D * S::EB);
-      const uint8_t* vs = vc + cell * (D * S::EB);
-#pragma unroll
-      for (int i = 0; i < S::HALF / 32; ++i) {
-        const int piece = i * 32 + lane, k = hf * 8 + piece / S::CPR;
-        const uint32_t to = dst + S::at(k, piece % S::CPR);
-        bool kt = true, vt = true;
-        if (!clean) {
-          kt = id >= 0;
-          vt = kt && seen_by_any(p, pos_lo, pos_hi, q.ctx, tok0 + k);
-        }
-        copy16(to, ks + i * 512, kt);
-        copy16(to + S::TILE, vs + i * 512, vt);
+  // Copies the group at keys [tok0, tok0 + TK) into a stage; `id` holds, in lanes
+  // base, base + 1, ..., the page of each run of 8 keys. A lane per box; rows past
+  // the cache arrive as zeros: missing pages.
+  const int box = min(16, bs);  // rows of a box
+  const int none = (int)(((int64_t)p.num_blocks * p.Hkv) << p.bs_log2);
+  auto copy_group = [&](int stage, int tok0, int id, int base) {
+    uint64_t* bar = &full[stage];
+    const int r = lane * box;  // this lane's first row
+    const int mine_id = __shfl_sync(0xffffffffu, id, base + (r >> 3) % S::GR);
+    if (lane == 0) sm100::mbar_arrive_expect_tx(bar, S::STAGE);
+    __syncwarp();
+    if (r >= TK) return;
+    const uint32_t dst = sm100::smem_u32(ring + stage * S::STAGE) +
+                         (S::CPR == 16 ? (r >> 4) * 4096 + (r & 15) * 128 : r * (S::CPR * 16));
+    const int row =
+        mine_id >= 0 ? (int)(((int64_t)mine_id * p.Hkv + hk) << p.bs_log2) + ((tok0 + r) & (bs - 1)) : none;
+    if constexpr (S::CPR == 16) {  // both halves of 16 rows, or each half of 8
+      for (int z = 0; z < (box == 16 ? 1 : 2); ++z) {
+        tma_load_3d(dst + z * 2048, &tk, bar, 0, row, z);
+        tma_load_3d(dst + z * 2048 + S::TILE, &tv, bar, 0, row, z);
       }
-      if constexpr (FP8) {
-        if (lane < 2)
-          copy8(dst + 2 * S::TILE + lane * 16 + hf * 8, (lane == 0 ? p.k_scale : p.v_scale) + cell,
-                id >= 0);
-      }
+    } else {
+      tma_load_2d(dst, &tk, bar, 0, row);
+      tma_load_2d(dst + S::TILE, &tv, bar, 0, row);
     }
+  };
+  // e4m3: this lane's scale bytes of the group, of K (low) and V, key lane;
+  // 127 (a scale of 1) where there is no page.
+  auto fetch_scales = [&](int tok0, int id, int base) -> int {
+    const int my = __shfl_sync(0xffffffffu, id, base + (lane >> 3) % S::GR);
+    if (my < 0) return 127 | 127 << 8;
+    const int64_t cell = (((int64_t)my * p.Hkv + hk) << p.bs_log2) + ((tok0 + lane) & (bs - 1));
+    return p.k_scale[cell] | p.v_scale[cell] << 8;
   };
 
   // Group n of this warp is v0 + warp + n WARPS and sits in stage n % STAGES.
   constexpr int AHEAD = S::STAGES - 1;
   const int first = v0 + warp;
   const int mine = v1 > first ? (v1 - first + WARPS - 1) / WARPS : 0;
-  int near = fetch_ids(first), far = fetch_ids(first + 16 * WARPS);
+  int near = fetch_ids(first), far = fetch_ids(first + BATCH * WARPS);
+  int scale_of[AHEAD + 1];  // scale bytes of the groups in flight
   auto copy_next = [&](int n) -> uint32_t {  // called for n = 0, 1, 2, ... in turn
-    if (n > 0 && n % 16 == 0) {
+    if (n > 0 && n % BATCH == 0) {
       near = far;
-      far = fetch_ids(first + (n + 16) * WARPS);
+      far = fetch_ids(first + (n + BATCH) * WARPS);
     }
-    const int a = __shfl_sync(0xffffffffu, near, 2 * (n % 16));
-    const int b = __shfl_sync(0xffffffffu, near, 2 * (n % 16) + 1);
-    if (n < mine) copy_group(n % S::STAGES, span.tile(first + n * WARPS) * TK, a, b);
-    copies_commit();  // a group of copies per n, empty past the end
-    return (a >= 0 ? 1u : 0u) | (b >= 0 ? 2u : 0u);
+    const int base = n % BATCH * S::GR;
+    if (n < mine) {
+      const int tok0 = span.tile(first + n * WARPS) * TK;
+      copy_group(n % S::STAGES, tok0, near, base);
+      if constexpr (FP8) scale_of[AHEAD] = fetch_scales(tok0, near, base);
+    }
+    return __ballot_sync(0xffffffffu, near >= 0) >> base & ((1u << S::GR) - 1u);
   };
-  uint32_t there = 0;  // two bits per group in flight: which halves have a page
+  // Which runs of 8 keys have a page, GR bits per group in flight.
+  uint32_t there = 0;
 #pragma unroll
-  for (int n = 0; n < AHEAD; ++n) there |= copy_next(n) << (2 * n);
+  for (int n = 0; n < AHEAD; ++n) {
+    there |= copy_next(n) << (S::GR * n);
+    if constexpr (FP8) scale_of[n] = scale_of[AHEAD];
+  }
 
   // ---------------------------------------------------------------- Q ----
   // B fragments: pair 8 h + g of the tile, its 4-element piece per k step.
@@ -319,91 +343,112 @@ paged_rows_kernel(const Params p) {
       for (int e = 0; e < 4; ++e) acc[h][j][e] = 0.f;
   }
 
-  // S^T of the group: sc[h][2 n + e] = key 8 n + g, pair 8 h + 2 t + e.
-  auto scores = [&](const uint8_t* kt, float (&sc)[NH][4]) {
+  // S^T of the group: sc[h][u][2 n + e] = key 16 u + 8 n + sigma(g), pair
+  // 8 h + 2 t + e.
+  auto scores = [&](const uint8_t* kt, float (&sc)[NH][NU][4]) {
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sc[h][e] = 0.f;
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[h][u][e] = 0.f;
 #pragma unroll
     for (int i = 0; i < S::NK; ++i) {
-      uint32_t k[2][4];
+      uint32_t k[NU][2][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) load_words(k[n], kt + S::at(8 * n + g, 4 * i + t));
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) load_words(k[u][n], kt + S::at(16 * u + 8 * n + sigma(g), 4 * i + t));
 #pragma unroll
       for (int w = 0; w < S::EK / 4; ++w) {
         const int st = i * (S::EK / 4) + w;
-        uint32_t a[4];  // keys g, 8 + g; then their second halves of the step
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          if constexpr (FP8) {
-            a[n] = cvt_e4m3x2_f16x2((uint16_t)(k[n][w] & 0xffff));
-            a[2 + n] = cvt_e4m3x2_f16x2((uint16_t)(k[n][w] >> 16));
-          } else {
-            a[n] = k[n][2 * w];
-            a[2 + n] = k[n][2 * w + 1];
+        for (int u = 0; u < NU; ++u) {
+          uint32_t a[4];  // keys g, 8 + g; then their second halves of the step
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            if constexpr (FP8) {
+              a[n] = cvt_e4m3x2_f16x2((uint16_t)(k[u][n][w] & 0xffff));
+              a[2 + n] = cvt_e4m3x2_f16x2((uint16_t)(k[u][n][w] >> 16));
+            } else {
+              a[n] = k[u][n][2 * w];
+              a[2 + n] = k[u][n][2 * w + 1];
+            }
           }
-        }
 #pragma unroll
-        for (int h = 0; h < NH; ++h)
-          mma16816<F16>(sc[h], a[0], a[1], a[2], a[3], qb[h][st][0], qb[h][st][1]);
+          for (int h = 0; h < NH; ++h)
+            mma16816<F16>(sc[h][u], a[0], a[1], a[2], a[3], qb[h][st][0], qb[h][st][1]);
+        }
       }
     }
   };
 
-  // Weights of the group's keys as B fragments of O^T: pb[h][n] = pair 8 h + g,
-  // keys 8 n + 2 t, 8 n + 2 t + 1. Scores go to log2 units, to -inf for keys
-  // that a row does not see.
-  auto weights = [&](const uint8_t* scales, float (&sc)[NH][4], int tok0, uint32_t pages,
-                     uint32_t (&pb)[NH][2]) {
-    float ev[2] = {0.f, 0.f};
+  // Weights of the group's keys as B fragments of O^T: pb[h][u][n] = pair 8 h + g,
+  // rows 16 u + 8 n + 2 t and + 1. Scores go to log2 units, to -inf for keys that
+  // a row does not see.
+  auto weights = [&](int scale, float (&sc)[NH][NU][4], int tok0, uint32_t pages,
+                     uint32_t (&pb)[NH][NU][2]) {
+    float ev[NU][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      float f = 1.f, bad = 0.f;
-      if constexpr (FP8) {
-        const int kb = scales[8 * n + g], vb = scales[16 + 8 * n + g];
-        f = __uint_as_float((uint32_t)kb << 23);  // 255, e8m0's NaN, gives infinity here
-        bad = f - f;                              // and NaN here
-        ev[n] = vb == 255 ? __int_as_float(0x7fc00000)
-                          : __uint_as_float(0x4b000000u | vb) - (8388608.f + 127.f);
-      }
-#pragma unroll
-      for (int h = 0; h < NH; ++h)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          sc[h][2 * n + e] =
-              FP8 ? fmaf(sc[h][2 * n + e] * fac[h][e], f, bad) : sc[h][2 * n + e] * fac[h][e];
-    }
-    if (pages != 3u || !all_seen(tok0)) {
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const int j = tok0 + 8 * n + g;
-        const bool page = (pages >> n) & 1;
+        float f = 1.f, bad = 0.f;
+        ev[u][n] = 0.f;
+        if constexpr (FP8) {
+          const int b = __shfl_sync(0xffffffffu, scale, 16 * u + 8 * n + sigma(g));
+          f = __uint_as_float((uint32_t)(b & 0xff) << 23);  // 255, e8m0's NaN, gives infinity here
+          bad = f - f;                                      // and NaN here
+          ev[u][n] = (b >> 8) == 255 ? __int_as_float(0x7fc00000)
+                                     : __uint_as_float(0x4b000000u | (b >> 8)) - (8388608.f + 127.f);
+        }
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (!page || !sees(p, pos[h][e], q.ctx, j)) sc[h][2 * n + e] = -INFINITY;
-        if (!page || !seen_by_any(p, pos_lo, pos_hi, q.ctx, j)) ev[n] = 0.f;
+            sc[h][u][2 * n + e] = FP8 ? fmaf(sc[h][u][2 * n + e] * fac[h][e], f, bad)
+                                      : sc[h][u][2 * n + e] * fac[h][e];
       }
+    if (pages != (1u << S::GR) - 1u || !all_seen(tok0)) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int j = tok0 + 16 * u + 8 * n + sigma(g);
+          const bool page = (pages >> (2 * u + n)) & 1;
+#pragma unroll
+          for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!page || !sees(p, pos[h][e], q.ctx, j)) sc[h][u][2 * n + e] = -INFINITY;
+          if (!page || !seen_by_any(p, pos_lo, pos_hi, q.ctx, j)) ev[u][n] = 0.f;
+        }
     }
     bool raise = false;
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          raise |= sc[h][2 * n + e] > m[h][e] + RAISE;
-          if constexpr (FP8) raise |= sc[h][2 * n + e] + ev[n] > mw[h][e] + RAISE;
-        }
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            raise |= sc[h][u][2 * n + e] > m[h][e] + RAISE;
+            if constexpr (FP8) raise |= sc[h][u][2 * n + e] + ev[u][n] > mw[h][e] + RAISE;
+          }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float a = fmaxf(m[h][e], fmaxf(sc[h][e], sc[h][2 + e]));
-          float b = FP8 ? fmaxf(mw[h][e], fmaxf(sc[h][e] + ev[0], sc[h][2 + e] + ev[1])) : 0.f;
+          float a = m[h][e], b = mw[h][e];
+#pragma unroll
+          for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              a = fmaxf(a, sc[h][u][2 * n + e]);
+              if constexpr (FP8) b = fmaxf(b, sc[h][u][2 * n + e] + ev[u][n]);
+            }
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) {
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
@@ -431,29 +476,32 @@ paged_rows_kernel(const Params p) {
         mmw[e] = mw[h][e] == -INFINITY ? 0.f : mw[h][e] - LIFT;
       }
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const float p0 = sm100::ex2(sc[h][2 * n] - mm[0]), p1 = sm100::ex2(sc[h][2 * n + 1] - mm[1]);
-        l[h][0] += p0;
-        l[h][1] += p1;
-        uint32_t w;
-        if constexpr (FP8)
-          w = sm100::pack_f16(sm100::ex2(sc[h][2 * n] + (ev[n] - mmw[0])),
-                              sm100::ex2(sc[h][2 * n + 1] + (ev[n] - mmw[1])));
-        else
-          w = F16 ? sm100::pack_f16(p0, p1) : sm100::pack_bf16(p0, p1);
-        pb[h][n] = transpose8x8(w);
-      }
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const float x0 = sc[h][u][2 * n], x1 = sc[h][u][2 * n + 1];
+          const float p0 = sm100::ex2(x0 - mm[0]), p1 = sm100::ex2(x1 - mm[1]);
+          l[h][0] += p0;
+          l[h][1] += p1;
+          uint32_t w;
+          if constexpr (FP8)
+            w = sm100::pack_f16(sm100::ex2(x0 + (ev[u][n] - mmw[0])), sm100::ex2(x1 + (ev[u][n] - mmw[1])));
+          else
+            w = F16 ? sm100::pack_f16(p0, p1) : sm100::pack_bf16(p0, p1);
+          pb[h][u][n] = transpose8x8(w);
+        }
     }
   };
 
-  auto weigh_v = [&](const uint8_t* vt, const uint32_t (&pb)[NH][2]) {
+  auto weigh_v = [&](const uint8_t* vt, const uint32_t (&pb)[NH][NU][2]) {
 #pragma unroll
-    for (int i = 0; i < S::NV; ++i) {
-      uint32_t vw[4][S::WV];  // keys 2t, 2t + 1, 8 + 2t, 9 + 2t
+    for (int ui = 0; ui < NU * S::NV; ++ui) {
+      const int u = ui / S::NV, i = ui % S::NV;
+      uint32_t vw[4][S::WV];  // the keys of rows 2t, 2t + 1, 8 + 2t, 9 + 2t
       const int byte = (8 * i + g) * (S::EV * S::EB);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        load_words(vw[e], vt + S::at((e >> 1) * 8 + 2 * t + (e & 1), byte / 16) + byte % 16);
+        load_words(vw[e], vt + S::at(16 * u + (e >> 1) * 8 + sigma(2 * t + (e & 1)), byte / 16) + byte % 16);
       // m-tile j's rows g and 8 + g are dims 2 j' and 2 j' + 1 of the lane's run.
 #pragma unroll
       for (int w = 0; w < S::WV; ++w) {
@@ -472,8 +520,8 @@ paged_rows_kernel(const Params p) {
           const uint32_t h3 = cvt_e4m3x2_f16x2((uint16_t)(hi1 >> 16));
 #pragma unroll
           for (int h = 0; h < NH; ++h) {
-            mma16816<F16>(acc[h][j], l0, l1, l2, l3, pb[h][0], pb[h][1]);
-            mma16816<F16>(acc[h][j + 1], h0, h1, h2, h3, pb[h][0], pb[h][1]);
+            mma16816<F16>(acc[h][j], l0, l1, l2, l3, pb[h][u][0], pb[h][u][1]);
+            mma16816<F16>(acc[h][j + 1], h0, h1, h2, h3, pb[h][u][0], pb[h][u][1]);
           }
         } else {
           const int j = (i * S::EV + 2 * w) / 2;
@@ -481,25 +529,42 @@ paged_rows_kernel(const Params p) {
           const uint32_t x2 = __byte_perm(c, d, 0x5410), x3 = __byte_perm(c, d, 0x7632);
 #pragma unroll
           for (int h = 0; h < NH; ++h)
-            mma16816<F16>(acc[h][j], x0, x1, x2, x3, pb[h][0], pb[h][1]);
+            mma16816<F16>(acc[h][j], x0, x1, x2, x3, pb[h][u][0], pb[h][u][1]);
         }
       }
     }
   };
 
+  bool ok = true;
   for (int n = 0; n < mine; ++n) {
-    copies_wait<AHEAD - 1>();  // this lane's copies of group n are in
-    __syncwarp();              // every lane's are, and group n - 1 has been read by all
-    there |= copy_next(n + AHEAD) << (2 * AHEAD);
-    const uint8_t* st = ring + (n % S::STAGES) * S::STAGE;
-    float sc[NH][4];
+    const int tok0 = span.tile(first + n * WARPS) * TK;
+    if (!sm100::mbar_wait_warp(&full[n % S::STAGES], (n / S::STAGES) & 1, 0x601)) { ok = false; break; }
+    // (Group n - 1 has been read by all lanes: its loads fed MMAs before the
+    // vote above.)
+    there |= copy_next(n + AHEAD) << (S::GR * AHEAD);
+    uint8_t* st = ring + (n % S::STAGES) * S::STAGE;
+    if (!all_seen(tok0)) {
+      // V rows that no row of the tile sees: what such cells hold must not meet
+      // a weight of 0.
+      const int k = lane % TK;
+      if (!seen_by_any(p, pos_lo, pos_hi, q.ctx, tok0 + k))
+        for (int c = lane / TK; c < S::CPR; c += 32 / TK)
+          *reinterpret_cast<uint4*>(st + S::TILE + S::at(k, c)) = make_uint4(0u, 0u, 0u, 0u);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next boxes
+      __syncwarp();
+    }
+    float sc[NH][NU][4];
     scores(st, sc);
-    uint32_t pb[NH][2];
-    weights(st + 2 * S::TILE, sc, span.tile(first + n * WARPS) * TK, there & 3u, pb);
+    uint32_t pb[NH][NU][2];
+    weights(FP8 ? scale_of[0] : 0, sc, tok0, there & ((1u << S::GR) - 1u), pb);
     weigh_v(st + S::TILE, pb);
-    there >>= 2;
+    there >>= S::GR;
+    if constexpr (FP8) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) scale_of[i] = scale_of[i + 1];
+    }
   }
-  copies_wait<0>();
+  (void)ok;  // a wait that gave up has left its code; the rest is skipped
   __syncthreads();  // the merge reuses the rings
 
   // ------------------------------------------------------------- merge ----
@@ -569,15 +634,49 @@ paged_rows_kernel(const Params p) {
   }
 }
 
+// The cache as rows: 64- or 128-byte rows, or the two 128-byte halves of
+// 256-byte ones; a box is the rows of a group that one page holds.
+template <bool FP8, int D>
+static int make_map(CUtensorMap* map, const void* base, const Params& p, bool bf16) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled unavailable (no CUDA driver?)");
+    return LSB_ERR_CUDA;
+  }
+  using S = Shape<FP8, D>;
+  const int inner = FP8 ? D : 64, rank = S::CPR == 16 ? 3 : 2;
+  cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)(((int64_t)p.num_blocks * p.Hkv) << p.bs_log2), 2};
+  cuuint64_t strides[2] = {(cuuint64_t)(D * S::EB), 128};
+  // (pages of 8: a box per half row, whose 16-row halves two boxes share)
+  cuuint32_t box[3] = {(cuuint32_t)inner, (cuuint32_t)(p.bs_log2 >= 4 ? 16 : 8), p.bs_log2 >= 4 ? 2u : 1u};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type = FP8    ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = enc(map, type, rank, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   S::CPR == 4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LSB_ERR_CUDA;
+  }
+  return LSB_OK;
+}
+
 template <typename T, bool FP8, int D, int NH>
 static int launch_tile(const Params& p, cudaStream_t st) {
   constexpr int smem = smem_bytes<FP8, D, NH>();
+  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  CUtensorMap mk, mv;
+  if (int rc = make_map<FP8, D>(&mk, p.k_cache, p, BF)) return rc;
+  if (int rc = make_map<FP8, D>(&mv, p.v_cache, p, BF)) return rc;
   auto kern = paged_rows_kernel<T, FP8, D, NH>;
   static SmemLimit limit;
   if (int rc = limit.ensure(kern, smem, "paged_attn smem attribute")) return rc;
   const int64_t pairs = (int64_t)p.max_q * p.G;
   const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)((pairs + 8 * NH - 1) / (8 * NH)), (unsigned)p.S);
-  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(WARPS * 32), smem, st, p), "paged_attn");
+  LSB_CUDA_OK(launch_kernel(kern, grid, dim3(WARPS * 32), smem, st, mk, mv, p), "paged_attn");
   return LSB_OK;
 }
 
@@ -592,15 +691,15 @@ static int launch(const Params& p, cudaStream_t st) {
 
 }  // namespace rows
 
-bool rows_eligible(const Params& p, int dtype, bool kv_fp8) {
+bool rows_eligible(const Params& p, int dtype) {
   if (dtype != LSB_DTYPE_BF16 && dtype != LSB_DTYPE_F16) return false;
   if ((p.D != 64 && p.D != 128) || p.bs_log2 < 3) return false;
-  // q rows are read in 8-byte pieces, the cache in 16-byte ones, the scales of
-  // 8 keys at a time.
+  // q rows are read in 8-byte pieces; the cache's rows are a 32-bit TMA
+  // coordinate, its base 16-byte aligned.
   auto at = [](const void* x, uintptr_t a) { return (reinterpret_cast<uintptr_t>(x) & (a - 1)) == 0; };
   if (!at(p.q, 8) || p.sq_t % 4 != 0 || p.sq_h % 4 != 0) return false;
   if (!at(p.k_cache, 16) || !at(p.v_cache, 16)) return false;
-  if (kv_fp8 && (!at(p.k_scale, 8) || !at(p.v_scale, 8))) return false;
+  if ((((int64_t)p.num_blocks * p.Hkv) << p.bs_log2) > 0x7fffffff) return false;
   return (int64_t)p.max_q * p.G / 8 < 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff;
 }
 
@@ -615,4 +714,7 @@ int launch_rows(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
 }
 
 }  // namespace pa
+
+int paged_attn_rows_device_error(bool reset) { return sm100::tu_device_error(reset); }
+
 }  // namespace lsb
