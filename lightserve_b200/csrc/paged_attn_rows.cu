@@ -128,9 +128,9 @@ struct Shape {
   static constexpr int TILE = TK * CPR * 16;       // bytes of a group's K (and V)
   static constexpr int STAGE = 2 * TILE;
   // Groups in flight per warp, sized so that an SM holds about 190 KB of ring.
-  static constexpr int STAGES = FP8 ? (D == 64 ? 3 : 2) : (D == 64 ? 4 : 3);
+  static constexpr int STAGES = FP8 ? 2 : (D == 64 ? 4 : 3);
   static constexpr int ctas(int nh) {
-    return FP8 ? (D == 64 ? (nh == 1 ? 4 : 3) : (nh == 3 ? 2 : 3)) : (D == 64 ? 3 : 2);
+    return FP8 ? (D == 64 ? (nh == 1 ? 5 : 3) : (nh == 3 ? 2 : 3)) : (D == 64 ? 3 : 2);
   }
   // Byte offset of 16-byte piece c of key k's row in its tile, as the boxes of
   // up to 16 rows and their swizzle leave it (256-byte rows come in two halves
@@ -149,7 +149,7 @@ constexpr int smem_bytes() {
   return (ring > merge ? ring : merge) + 1024;  // slack for 1024-byte alignment
 }
 
-template <typename T, bool FP8, int D, int NH>
+template <typename T, bool FP8, int D, int NH, bool ONE>
 __global__ void __launch_bounds__(WARPS * 32, (Shape<FP8, D>::ctas(NH)))
 paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                   const Params p) {
@@ -161,7 +161,10 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   wait_prerequisites();
   using S = Shape<FP8, D>;
   constexpr bool F16 = FP8 || std::is_same<T, __half>::value;  // MMA operand type
-  constexpr int R = 8 * NH, TK = S::TK, NU = S::NU;
+  // NE: of a lane's pairs 8 h + 2 t and + 1, those that can be in use (ONE: the
+  // call has one pair per cache head, plain decode).
+  constexpr int R = 8 * NH, TK = S::TK, NU = S::NU, NE = ONE ? 1 : 2;
+  static_assert(!ONE || NH == 1, "one pair fits one block");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (sm100::smem_u32(smem_raw) & 1023)) & 1023);
   __shared__ uint64_t bars[WARPS][S::STAGES];  // a group's boxes have arrived
@@ -274,8 +277,8 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   uint32_t qb[NH][S::STEPS][2];
   // Of pairs 8 h + 2 t and 8 h + 2 t + 1, whose scores this lane holds: the
   // score's factor (scale log2(e), and the row's power of two) and position.
-  float fac[NH][2];
-  int pos[NH][2];
+  float fac[NH][NE];
+  int pos[NH][NE];
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
     const int pr = tile * R + h * 8 + g;
@@ -319,7 +322,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       }
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {  // lane 4 (2 t + e) holds pair 8 h + 2 t + e
+    for (int e = 0; e < NE; ++e) {  // lane 4 (2 t + e) holds pair 8 h + 2 t + e
       fac[h][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * t + e));
       const int pe = tile * R + h * 8 + 2 * t + e;
       pos[h][e] = pe < pairs ? q.pos0 + pe / p.G : -1;  // position -1 sees nothing
@@ -329,11 +332,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   // ----------------------------------------------------------- compute ----
   // Running maxima m (of scores) and mw (of scores + V exponents), held as the
   // thresholds that raise them; sums and outputs are relative to them.
-  float m[NH][2], mw[NH][2], l[NH][2], acc[NH][S::MT][4];
+  float m[NH][NE], mw[NH][NE], l[NH][NE], acc[NH][S::MT][4];
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < NE; ++e) {
       m[h][e] = mw[h][e] = -INFINITY;
       l[h][e] = 0.f;
     }
@@ -346,12 +349,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   // S^T of the group: sc[h][u][2 n + e] = key 16 u + 8 n + sigma(g), pair
   // 8 h + 2 t + e.
   auto scores = [&](const uint8_t* kt, float (&sc)[NH][NU][4]) {
+    float odd[NH][NU][4];  // odd k steps: half as long a chain of MMAs
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[h][u][e] = 0.f;
+        for (int e = 0; e < 4; ++e) sc[h][u][e] = odd[h][u][e] = 0.f;
 #pragma unroll
     for (int i = 0; i < S::NK; ++i) {
       uint32_t k[NU][2][4];
@@ -377,10 +381,17 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
           }
 #pragma unroll
           for (int h = 0; h < NH; ++h)
-            mma16816<F16>(sc[h][u], a[0], a[1], a[2], a[3], qb[h][st][0], qb[h][st][1]);
+            mma16816<F16>(st % 2 == 0 ? sc[h][u] : odd[h][u], a[0], a[1], a[2], a[3], qb[h][st][0],
+                          qb[h][st][1]);
         }
       }
     }
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[h][u][e] += odd[h][u][e];
   };
 
   // Weights of the group's keys as B fragments of O^T: pb[h][u][n] = pair 8 h + g,
@@ -405,7 +416,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int e = 0; e < NE; ++e)
             sc[h][u][2 * n + e] = FP8 ? fmaf(sc[h][u][2 * n + e] * fac[h][e], f, bad)
                                       : sc[h][u][2 * n + e] * fac[h][e];
       }
@@ -419,7 +430,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
           for (int h = 0; h < NH; ++h)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < NE; ++e)
               if (!page || !sees(p, pos[h][e], q.ctx, j)) sc[h][u][2 * n + e] = -INFINITY;
           if (!page || !seen_by_any(p, pos_lo, pos_hi, q.ctx, j)) ev[u][n] = 0.f;
         }
@@ -432,7 +443,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          for (int e = 0; e < NE; ++e) {
             raise |= sc[h][u][2 * n + e] > m[h][e] + RAISE;
             if constexpr (FP8) raise |= sc[h][u][2 * n + e] + ev[u][n] > mw[h][e] + RAISE;
           }
@@ -440,7 +451,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
       for (int h = 0; h < NH; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < NE; ++e) {
           float a = m[h][e], b = mw[h][e];
 #pragma unroll
           for (int u = 0; u < NU; ++u)
@@ -469,9 +480,9 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
-      float mm[2], mmw[2];
+      float mm[NE], mmw[NE];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < NE; ++e) {
         mm[e] = m[h][e] == -INFINITY ? 0.f : m[h][e] - LIFT;
         mmw[e] = mw[h][e] == -INFINITY ? 0.f : mw[h][e] - LIFT;
       }
@@ -480,12 +491,13 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const float x0 = sc[h][u][2 * n], x1 = sc[h][u][2 * n + 1];
-          const float p0 = sm100::ex2(x0 - mm[0]), p1 = sm100::ex2(x1 - mm[1]);
+          const float p0 = sm100::ex2(x0 - mm[0]), p1 = ONE ? 0.f : sm100::ex2(x1 - mm[NE - 1]);
           l[h][0] += p0;
-          l[h][1] += p1;
+          if constexpr (!ONE) l[h][NE - 1] += p1;
           uint32_t w;
           if constexpr (FP8)
-            w = sm100::pack_f16(sm100::ex2(x0 + (ev[u][n] - mmw[0])), sm100::ex2(x1 + (ev[u][n] - mmw[1])));
+            w = sm100::pack_f16(sm100::ex2(x0 + (ev[u][n] - mmw[0])),
+                                ONE ? 0.f : sm100::ex2(x1 + (ev[u][n] - mmw[NE - 1])));
           else
             w = F16 ? sm100::pack_f16(p0, p1) : sm100::pack_bf16(p0, p1);
           pb[h][u][n] = transpose8x8(w);
@@ -575,7 +587,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
 #pragma unroll
   for (int h = 0; h < NH; ++h)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < NE; ++e) {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], o);
       const int r = h * 8 + 2 * t + e;
@@ -664,14 +676,14 @@ static int make_map(CUtensorMap* map, const void* base, const Params& p, bool bf
   return LSB_OK;
 }
 
-template <typename T, bool FP8, int D, int NH>
+template <typename T, bool FP8, int D, int NH, bool ONE>
 static int launch_tile(const Params& p, cudaStream_t st) {
   constexpr int smem = smem_bytes<FP8, D, NH>();
   constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
   CUtensorMap mk, mv;
   if (int rc = make_map<FP8, D>(&mk, p.k_cache, p, BF)) return rc;
   if (int rc = make_map<FP8, D>(&mv, p.v_cache, p, BF)) return rc;
-  auto kern = paged_rows_kernel<T, FP8, D, NH>;
+  auto kern = paged_rows_kernel<T, FP8, D, NH, ONE>;
   static SmemLimit limit;
   if (int rc = limit.ensure(kern, smem, "paged_attn smem attribute")) return rc;
   const int64_t pairs = (int64_t)p.max_q * p.G;
@@ -682,10 +694,12 @@ static int launch_tile(const Params& p, cudaStream_t st) {
 
 template <typename T, bool FP8, int D>
 static int launch(const Params& p, cudaStream_t st) {
-  switch (rows_tile((int64_t)p.max_q * p.G)) {
-    case 8: return launch_tile<T, FP8, D, 1>(p, st);
-    case 16: return launch_tile<T, FP8, D, 2>(p, st);
-    default: return launch_tile<T, FP8, D, 3>(p, st);
+  const int64_t pairs = (int64_t)p.max_q * p.G;
+  if (pairs == 1) return launch_tile<T, FP8, D, 1, true>(p, st);
+  switch (rows_tile(pairs)) {
+    case 8: return launch_tile<T, FP8, D, 1, false>(p, st);
+    case 16: return launch_tile<T, FP8, D, 2, false>(p, st);
+    default: return launch_tile<T, FP8, D, 3, false>(p, st);
   }
 }
 
