@@ -46,11 +46,12 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale, dtype, index):
 
 
 def _window_args(window, num_sinks):
-    """(window, num_sinks) as the C entry takes them (0: no window)."""
+    """(window, num_sinks) as the C entry takes them (0: no window; both held at
+    2^31, past every position)."""
     assert window is None or int(window) > 0, f"window must be positive, got {window}"
     assert int(num_sinks) >= 0, f"num_sinks must not be negative, got {num_sinks}"
     assert window is not None or not num_sinks, "num_sinks needs a window (without one every key is visible)"
-    return int(window or 0), int(num_sinks)
+    return min(int(window or 0), 1 << 31), min(int(num_sinks), 1 << 31)
 
 
 def paged_chunk_workspace(q_shape, num_seqs: int, max_seqlen_q: int, num_kv_heads: int,

@@ -79,6 +79,16 @@ def test_windows(window, sinks, dtype, quantised, impl):
     _check(b, window, sinks, IMPLS[impl])
 
 
+@pytest.mark.parametrize("new", [[1, 1], [140, 9]])
+def test_windows_past_every_position(new):
+    b = R.build([3000, 77], new, 2, 2, 128, 16, BF16, seed=4)
+    plain = _run(b)
+    for window, sinks in (((1 << 31) - 1, 0), (1 << 62, 1 << 62), (1 << 70, 1 << 70), (5, 1 << 62)):
+        out, _ = _check(b, min(window, 1 << 31), min(sinks, 1 << 31))
+        assert torch.equal(_run(b, window, sinks), out)
+    assert torch.equal(_run(b, 1 << 62, 1 << 62), plain)
+
+
 @pytest.mark.parametrize("quantised", [False, True])
 @pytest.mark.parametrize("H,G", [(1, 1), (3, 1), (1, 2), (2, 3), (1, 7), (2, 8), (1, 16), (1, 33)])
 @pytest.mark.parametrize("new", [1, 6, 150])

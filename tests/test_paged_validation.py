@@ -177,3 +177,12 @@ def test_workspace_follows_the_window():
     short = paged_chunk_workspace((1, 8, 128), 1, 1, 8, 4096, 16, "cpu", 64, 4)
     many = paged_chunk_workspace((70000, 8, 128), 8, 65536, 8, 4096, 16, "cpu")
     assert full.numel() > short.numel() > many.numel() == 1
+
+
+@pytest.mark.parametrize("window,sinks", [(1 << 62, 1 << 62), (1 << 70, 0), (64, 1 << 62), (1 << 62, 3)])
+def test_workspace_of_windows_past_every_position(window, sinks):
+    """Sizes whose sum leaves 64 bits still ask for the scratch of the whole context."""
+    full = paged_chunk_workspace((1, 8, 128), 1, 1, 8, 4096, 16, "cpu")
+    assert paged_chunk_workspace((1, 8, 128), 1, 1, 8, 4096, 16, "cpu", window, sinks).numel() == full.numel()
+    raw = min(window, (1 << 63) - 1), sinks
+    assert _lib.load().lsb_paged_attn_workspace_size(1, 1, 1, 8, 8, 128, 4096, 16, *raw) == 4 * full.numel()
