@@ -547,10 +547,14 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
     }
   };
 
-  bool ok = true;
   for (int n = 0; n < mine; ++n) {
     const int tok0 = span.tile(first + n * WARPS) * TK;
-    if (!sm100::mbar_wait_warp(&full[n % S::STAGES], (n / S::STAGES) & 1, 0x601)) { ok = false; break; }
+    if (!sm100::mbar_wait_warp(&full[n % S::STAGES], (n / S::STAGES) & 1, 0x601)) {
+      // The error word is set; no copy may be in flight when the rings are reused.
+      for (int i = n; i < min(mine, n + AHEAD); ++i)
+        sm100::mbar_wait_warp(&full[i % S::STAGES], (i / S::STAGES) & 1, 0x601);
+      break;
+    }
     // (Group n - 1 has been read by all lanes: its loads fed MMAs before the
     // vote above.)
     there |= copy_next(n + AHEAD) << (S::GR * AHEAD);
@@ -576,7 +580,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       for (int i = 0; i < AHEAD; ++i) scale_of[i] = scale_of[i + 1];
     }
   }
-  (void)ok;  // a wait that gave up has left its code; the rest is skipped
   __syncthreads();  // the merge reuses the rings
 
   // ------------------------------------------------------------- merge ----
