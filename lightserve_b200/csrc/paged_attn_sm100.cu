@@ -264,11 +264,12 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     return id >= 0 && id < p.num_blocks ? id : -1;
   };
 
-  // Register split, 384 threads x 168 at launch: 128 x 96 + 256 x 200 = 63,488
-  // of 64,512. e4m3: 512 x 128 at launch: 128 x (48 + 80) + 256 x 192 = 65,536.
+  // Register split, 384 threads x 168 at launch: 128 x 56 + 256 x 224 = 64,512
+  // (with 200 the softmax spilled: one chunk of 8192 tokens, D 128, 229 us against
+  // 222). e4m3: 512 x 128 at launch: 128 x (48 + 80) + 256 x 192 = 65,536.
   if (warp == 0) {
     // ------------------------------------------------------------- loads --
-    reg_dealloc<FP8 ? 48 : 96>();
+    reg_dealloc<FP8 ? 48 : 56>();
     if (lane == 0) {
       const int tokens = w.R / p.G;
 #pragma unroll
@@ -367,7 +368,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     // it computed every descriptor outside the uniform registers, which paced the
     // loop: one chunk of 8192 tokens, 16 heads of 128, took 240 us against 229
     // (e4m3 325 against 281).
-    reg_dealloc<FP8 ? 48 : 96>();
+    reg_dealloc<FP8 ? 48 : 56>();
     constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, FMT, 0, 0);
     constexpr uint32_t IDESC_PV = idesc_f16(BM, D, FMT, 0, 1);
     const uint32_t q_lo = desc_lo(sQ, 16), k_lo = desc_lo(sK, 16), v_lo = desc_lo(sV, ATOM);
@@ -429,10 +430,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       if (j + 1 < w.nkv) mma_commit_warp(&k_empty[(j + 1) % NS]);
     }
   } else if (warp < 4) {
-    reg_dealloc<FP8 ? 48 : 96>();  // idle members of the first warpgroup
+    reg_dealloc<FP8 ? 48 : 56>();  // idle members of the first warpgroup
   } else if (warp < 12) {
     // ----------------------------------------------------------- softmax --
-    reg_alloc<FP8 ? 192 : 200>();
+    reg_alloc<FP8 ? 192 : 224>();
     const int t = (warp >> 2) - 1;
     const int row = threadIdx.x - 128 * (t + 1);  // TMEM lane
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
