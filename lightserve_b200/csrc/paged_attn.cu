@@ -11,59 +11,69 @@ namespace lsb {
 namespace pa {
 
 // ------------------------------------------------------- CUDA-core kernel --
-// One CTA: a query tile of SR = 16 pairs of one (sequence, cache head) and one
-// chunk of its keys; each of 4 warps owns 4 pairs. K and V tiles of STK = 32
-// keys are staged in shared memory as fp32 (dequantised there). Scores: lane =
-// key, so a K row is read once as float4s (row stride D + 4: conflict-free)
-// for 4 pairs whose q values are broadcast reads, 16 FMAs per 5 shared loads.
-// P V: lane = dim, each V element serving the warp's 4 pairs. All arithmetic is
-// fp32, as the fp32 model's parity with the reference needs (tensor-core TF32
-// does not reach it).
-constexpr int SR = 16;
+// One CTA: a query tile of 4 ROWS pairs of one (sequence, cache head) and one
+// chunk of its keys; its 4 warps own ROWS pairs each. K and V tiles of STK = 32
+// keys are staged in shared memory as fp32 (dequantised there; ROWS = 1: from
+// registers that were loaded a tile ahead). Scores: lane = key, so a K row is read
+// once as float4s (row stride D + 4: conflict-free) for ROWS pairs whose q values
+// are broadcast reads. P V: lane = dim, each V element serving the warp's pairs.
+// All arithmetic is fp32, as the fp32 model's parity with the reference needs
+// (tensor-core TF32 does not reach it).
+// ROWS = 1 serves up to 4 pairs (a tile of 16 took 197 us against 91 for 4
+// sequences of 2000-9000 fp32 keys, 8 cache heads of 128, 4 pairs: 38% of HBM);
+// 8, where half the CTAs still fill the GPU: shared-memory reads, 4 + ROWS
+// wavefronts per 4 ROWS FMAs of a warp, and issue slots bound it (4 chunks of
+// 300-700 tokens over 1000-4000, 8 x 2 heads of 128: 1650 us, 19 TFLOP/s, against
+// 2010 with 4; three short prompts 19 against 13).
 constexpr int STK = 32;
 constexpr int S_WARPS = 4;
-constexpr int S_ROWS = SR / S_WARPS;
+static int simt_rows(int64_t S, int64_t Hkv, int64_t pairs) {
+  if (pairs <= 4) return 1;
+  return pairs > 16 && S * Hkv * ((pairs + 31) / 32) >= 2 * 148 ? 8 : 4;
+}
+
+// Four elements of a cached row as they are stored; `left` of them exist.
+template <typename KV>
+struct alignas(4 * sizeof(KV)) Quad {
+  KV e[4];
+};
 
 template <typename KV>
-__device__ __forceinline__ void load4(const KV* p, bool vec, int left, float (&f)[4]) {
-  if constexpr (std::is_same<KV, uint8_t>::value) {
-    if (vec) {
-      e4m3x4_to_float(*reinterpret_cast<const uint32_t*>(p), f);
-      return;
-    }
+__device__ __forceinline__ Quad<KV> load4(const KV* p, bool vec, int left) {
+  if (vec) return *reinterpret_cast<const Quad<KV>*>(p);
+  Quad<KV> x = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      f[i] = i < left ? f16x2_to_float2(cvt_e4m3x2_f16x2(p[i])).x : 0.f;
-  } else {
-    if (vec) {
-      if constexpr (sizeof(KV) == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(p);
-        f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(p);
-        const KV* h = reinterpret_cast<const KV*>(&x);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = to_f(h[i]);
-      }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = i < left ? to_f(p[i]) : 0.f;
-  }
+  for (int i = 0; i < 4; ++i)
+    if (i < left) x.e[i] = p[i];
+  return x;
+}
+
+__device__ __forceinline__ float4 widen(const Quad<uint8_t>& x) {
+  float f[4];
+  e4m3x4_to_float(*reinterpret_cast<const uint32_t*>(x.e), f);
+  return make_float4(f[0], f[1], f[2], f[3]);
+}
+template <typename KV>
+__device__ __forceinline__ float4 widen(const Quad<KV>& x) {
+  return make_float4(to_f(x.e[0]), to_f(x.e[1]), to_f(x.e[2]), to_f(x.e[3]));
 }
 
 // DC: 32-dim columns per lane (head dim up to 32 DC).
-template <typename T, typename KV, int DC>
+template <typename T, typename KV, int DC, int ROWS>
 __global__ void __launch_bounds__(S_WARPS * 32)
 paged_simt_kernel(const Params p, const bool vec) {
   constexpr bool FP8 = std::is_same<KV, uint8_t>::value;
+  constexpr int SR = S_WARPS * ROWS;
+  // Staging: a warp's 8 keys of a tile, QL lanes per key, QPL quads per lane.
+  constexpr int QL = DC == 2 ? 16 : 32, QPL = DC == 8 ? 2 : 1;
+  constexpr int PASSES = STK / S_WARPS * QL / 32, N = PASSES * QPL;
+  constexpr bool AHEAD = ROWS == 1 && DC <= 4;  // (elsewhere its registers cost more than it hides)
   extern __shared__ float sm[];
   const int D = p.D, Dp = (D + 3) & ~3, ldk = Dp + 4;
   float* sQ = sm;                    // [SR][Dp]
   float* sK = sQ + SR * Dp;          // [STK][ldk]
   float* sV = sK + STK * ldk;        // [STK][Dp]
   float* sP = sV + STK * Dp;         // [SR][STK]
-  int* sOk = reinterpret_cast<int*>(sP + SR * STK);  // [STK]: the key was loaded
 
   const int s = blockIdx.z;
   const Seq q = load_seq(p, s);
@@ -88,15 +98,17 @@ paged_simt_kernel(const Params p, const bool vec) {
                                           (int64_t)(hk * p.G + r % p.G) * p.sq_h + d]);
     sQ[i] = x;
   }
-  int pos[S_ROWS];
+  // Pair r of this warp is pair r S_WARPS + warp of the tile.
+  int pos[ROWS];
 #pragma unroll
-  for (int r = 0; r < S_ROWS; ++r) {
-    const int pr = tile * SR + warp * S_ROWS + r;
+  for (int r = 0; r < ROWS; ++r) {
+    const int pr = tile * SR + r * S_WARPS + warp;
     pos[r] = pr < pairs ? q.pos0 + pr / p.G : -1;  // position -1 sees nothing
   }
-  float m[S_ROWS], l[S_ROWS], acc[S_ROWS][DC];
+  const bool live = tile * SR + warp < pairs;
+  float m[ROWS], l[ROWS], acc[ROWS][DC];
 #pragma unroll
-  for (int r = 0; r < S_ROWS; ++r) {
+  for (int r = 0; r < ROWS; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
@@ -105,46 +117,92 @@ paged_simt_kernel(const Params p, const bool vec) {
   const int32_t* bt = p.block_tables + (int64_t)s * p.max_blocks;
   const int bs = 1 << p.bs_log2;
 
+  // Page of key `lane` of span tile v; -1: none, or no row of the tile sees it.
+  auto fetch_id = [&](int v) -> int {
+    if (v >= v1) return -1;
+    const int key = span.tile(v) * STK + lane;
+    if (!seen_by_any(p, pos_lo, pos_hi, q.ctx, key)) return -1;
+    const int id = bt[key >> p.bs_log2];
+    return id >= 0 && id < p.num_blocks ? id : -1;
+  };
+  auto cell_of = [&](int id, int key) {
+    return (((int64_t)id * p.Hkv + hk) << p.bs_log2) + (key & (bs - 1));
+  };
+  // This thread's quads of a tile: n = pass QPL + u is key `row` + pass 32 / QL of
+  // the tile, dims from `dim` + 128 u on.
+  const int row = warp * (STK / S_WARPS) + lane / QL, dim = lane % QL * 4;
+  auto load = [&](const void* cache, int key0, int id, Quad<KV> (&x)[N]) {
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+      const int j = row + pass * (32 / QL), jd = __shfl_sync(0xffffffffu, id, j);
+#pragma unroll
+      for (int u = 0; u < QPL; ++u) {
+        const int d = dim + 128 * u;
+        x[pass * QPL + u] = Quad<KV>{};
+        if (jd >= 0 && d < D)
+          x[pass * QPL + u] = load4(static_cast<const KV*>(cache) + cell_of(jd, key0 + j) * D + d, vec, D - d);
+      }
+    }
+  };
+  // scale: the byte of key `lane`.
+  auto store = [&](float* dst, int ld, const Quad<KV> (&x)[N], int scale) {
+#pragma unroll
+    for (int pass = 0; pass < PASSES; ++pass) {
+      const int j = row + pass * (32 / QL);
+      const float f = FP8 ? e8m0_to_float(__shfl_sync(0xffffffffu, scale, j)) : 1.f;
+#pragma unroll
+      for (int u = 0; u < QPL; ++u) {
+        const int d = dim + 128 * u;
+        float4 y = widen(x[pass * QPL + u]);
+        if constexpr (FP8) y = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+        if (d < Dp) *reinterpret_cast<float4*>(dst + j * ld + d) = y;
+      }
+    }
+  };
+
+  Quad<KV> xk[N], xv[N];
+  int id = fetch_id(v0), id1 = fetch_id(v0 + 1), scales = 127 | 127 << 8;
+  auto load_tile = [&](int v, int ids) {
+    const int key0 = span.tile(v) * STK;
+    if constexpr (FP8) {
+      scales = 127 | 127 << 8;
+      if (ids >= 0) {
+        const int64_t cell = cell_of(ids, key0 + lane);
+        scales = p.k_scale[cell] | p.v_scale[cell] << 8;
+      }
+    }
+    load(p.k_cache, key0, ids, xk);
+    if constexpr (AHEAD) load(p.v_cache, key0, ids, xv);
+  };
+  if (AHEAD && v0 < v1) load_tile(v0, id);
   for (int v = v0; v < v1; ++v) {
     const int key0 = span.tile(v) * STK;
     __syncthreads();  // the previous tile (and, at first, nothing) has been read
-    const int d4 = Dp / 4;
-    for (int i = threadIdx.x; i < STK * d4; i += blockDim.x) {
-      const int j = i / d4, d = (i % d4) * 4, key = key0 + j;
-      const int blk =
-          seen_by_any(p, pos_lo, pos_hi, q.ctx, key) ? bt[key >> p.bs_log2] : -1;
-      const bool ok = blk >= 0 && blk < p.num_blocks;
-      float fk[4] = {0.f, 0.f, 0.f, 0.f}, fv[4] = {0.f, 0.f, 0.f, 0.f};
-      if (ok) {
-        const int64_t cell = ((int64_t)blk * p.Hkv + hk) * bs + (key & (bs - 1));
-        load4(static_cast<const KV*>(p.k_cache) + cell * D + d, vec, D - d, fk);
-        load4(static_cast<const KV*>(p.v_cache) + cell * D + d, vec, D - d, fv);
-        if constexpr (FP8) {
-          const float ks = e8m0_to_float(p.k_scale[cell]), vs = e8m0_to_float(p.v_scale[cell]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { fk[e] *= ks; fv[e] *= vs; }
-        }
-      }
-      *reinterpret_cast<float4*>(sK + j * ldk + d) = make_float4(fk[0], fk[1], fk[2], fk[3]);
-      *reinterpret_cast<float4*>(sV + j * Dp + d) = make_float4(fv[0], fv[1], fv[2], fv[3]);
-      if (d == 0) sOk[j] = ok;
-    }
+    if constexpr (!AHEAD) load_tile(v, id);
+    store(sK, ldk, xk, scales & 0xff);
+    if constexpr (!AHEAD) load(p.v_cache, key0, id, xv);
+    store(sV, Dp, xv, scales >> 8);
     __syncthreads();
-    float sc[S_ROWS] = {};
+    const bool key_ok = id >= 0;
+    id = id1;
+    id1 = fetch_id(v + 2);
+    if (AHEAD && v + 1 < v1) load_tile(v + 1, id);
+    if (!live) continue;
+    float sc[ROWS] = {};
+#pragma unroll 2
     for (int d = 0; d < Dp; d += 4) {
       const float4 kx = *reinterpret_cast<const float4*>(sK + lane * ldk + d);
 #pragma unroll
-      for (int r = 0; r < S_ROWS; ++r) {
-        const float4 qx = *reinterpret_cast<const float4*>(sQ + (warp * S_ROWS + r) * Dp + d);
+      for (int r = 0; r < ROWS; ++r) {
+        const float4 qx = *reinterpret_cast<const float4*>(sQ + (r * S_WARPS + warp) * Dp + d);
         sc[r] = fmaf(qx.x, kx.x, sc[r]);
         sc[r] = fmaf(qx.y, kx.y, sc[r]);
         sc[r] = fmaf(qx.z, kx.z, sc[r]);
         sc[r] = fmaf(qx.w, kx.w, sc[r]);
       }
     }
-    const bool key_ok = sOk[lane] != 0;
 #pragma unroll
-    for (int r = 0; r < S_ROWS; ++r) {
+    for (int r = 0; r < ROWS; ++r) {
       const float x = key_ok && sees(p, pos[r], q.ctx, key0 + lane) ? sc[r] * p.scale_log2 : -INFINITY;
       // A NaN score stays visible: fmaxf drops it, but exp2f below returns it.
       const float mx = fmaxf(m[r], warp_max(x));
@@ -155,14 +213,14 @@ paged_simt_kernel(const Params p, const bool vec) {
       l[r] = l[r] * a + e;  // per-lane partial sum
 #pragma unroll
       for (int c = 0; c < DC; ++c) acc[r][c] *= a;
-      sP[(warp * S_ROWS + r) * STK + lane] = e;
+      sP[(warp * ROWS + r) * STK + lane] = e;
     }
     __syncwarp();
     for (int j = 0; j < STK; j += 4) {
-      float4 pr[S_ROWS];
+      float4 pr[ROWS];
 #pragma unroll
-      for (int r = 0; r < S_ROWS; ++r)
-        pr[r] = *reinterpret_cast<const float4*>(sP + (warp * S_ROWS + r) * STK + j);
+      for (int r = 0; r < ROWS; ++r)
+        pr[r] = *reinterpret_cast<const float4*>(sP + (warp * ROWS + r) * STK + j);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -170,7 +228,7 @@ paged_simt_kernel(const Params p, const bool vec) {
           const int d = c * 32 + lane;
           const float vx = d < Dp ? sV[(j + e) * Dp + d] : 0.f;
 #pragma unroll
-          for (int r = 0; r < S_ROWS; ++r) {
+          for (int r = 0; r < ROWS; ++r) {
             const float pe = e == 0 ? pr[r].x : e == 1 ? pr[r].y : e == 2 ? pr[r].z : pr[r].w;
             acc[r][c] = fmaf(pe, vx, acc[r][c]);
           }
@@ -179,8 +237,8 @@ paged_simt_kernel(const Params p, const bool vec) {
     }
   }
 #pragma unroll
-  for (int r = 0; r < S_ROWS; ++r) {
-    const int pr = tile * SR + warp * S_ROWS + r;
+  for (int r = 0; r < ROWS; ++r) {
+    const int pr = tile * SR + r * S_WARPS + warp;
     if (pr >= pairs) continue;
     const int row = q.row0 + pr / p.G, h = hk * p.G + pr % p.G;
     const float lsum = warp_sum(l[r]);
@@ -203,13 +261,14 @@ paged_simt_kernel(const Params p, const bool vec) {
 }
 
 int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
-  const int Dp = (p.D + 3) & ~3;
-  const size_t smem = sizeof(float) * (SR * Dp + STK * (Dp + 4) + STK * Dp + SR * STK + STK);
+  const int Dp = (p.D + 3) & ~3, rows = simt_rows(p.S, p.Hkv, (int64_t)p.max_q * p.G);
+  const int SR = S_WARPS * rows;
+  const size_t smem = sizeof(float) * (SR * Dp + STK * (Dp + 4) + STK * Dp + SR * STK);
   const int64_t tiles = ((int64_t)p.max_q * p.G + SR - 1) / SR;
   LSB_CHECK_ARG(tiles <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff,
                 "paged_attn: %lld query tiles per head exceed 65535 (CUDA-core kernel)", (long long)tiles);
   const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)tiles, (unsigned)p.S);
-  auto go = [&](auto tag, auto kvtag, auto dc) -> int {
+  auto go = [&](auto tag, auto kvtag, auto dc, auto nr) -> int {
     using T = decltype(tag);
     using KV = decltype(kvtag);
     constexpr int DC = decltype(dc)::value;
@@ -217,7 +276,7 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
     const bool vec = p.D % 4 == 0 &&
                      ((reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) &
                       (4 * sizeof(KV) - 1)) == 0;
-    auto kern = paged_simt_kernel<T, KV, DC>;
+    auto kern = paged_simt_kernel<T, KV, DC, decltype(nr)::value>;
     static SmemLimit limit;
     if (smem > 48 * 1024)
       if (int rc = limit.ensure(kern, smem, "paged_attn smem attribute")) return rc;
@@ -225,10 +284,15 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
     LSB_CHECK_LAUNCH("paged_attn");
     return LSB_OK;
   };
+  auto by_rows = [&](auto tag, auto kvtag, auto dc) -> int {
+    if (rows == 1) return go(tag, kvtag, dc, std::integral_constant<int, 1>{});
+    if (rows == 4) return go(tag, kvtag, dc, std::integral_constant<int, 4>{});
+    return go(tag, kvtag, dc, std::integral_constant<int, 8>{});
+  };
   auto by_dim = [&](auto tag, auto kvtag) -> int {
-    if (p.D <= 64) return go(tag, kvtag, std::integral_constant<int, 2>{});
-    if (p.D <= 128) return go(tag, kvtag, std::integral_constant<int, 4>{});
-    return go(tag, kvtag, std::integral_constant<int, 8>{});
+    if (p.D <= 64) return by_rows(tag, kvtag, std::integral_constant<int, 2>{});
+    if (p.D <= 128) return by_rows(tag, kvtag, std::integral_constant<int, 4>{});
+    return by_rows(tag, kvtag, std::integral_constant<int, 8>{});
   };
   return LSB_DISPATCH_DTYPE(dtype, T, [&] {
     if (kv_fp8) return by_dim(T{}, uint8_t{});
@@ -317,8 +381,8 @@ int launch_combine(const Params& p, int rows_per_tile, int tk, int dtype, cudaSt
 
 // -------------------------------------------------------------- dispatch ---
 // How a call's keys are cut, from its sizes alone: with fewer query tiles
-// than the GPU holds CTAs (4 of them on each of a B200's 148 SMs for the
-// CUDA-core kernel), each tile's keys go to P CTAs of `chunk` keys.
+// than the GPU holds CTAs (8 on each of a B200's 148 SMs for the CUDA-core
+// kernel), each tile's keys go to P CTAs of `chunk` keys.
 struct Plan {
   int chunk, P;
 };
@@ -339,7 +403,8 @@ static int64_t max_visible(int64_t max_q, int64_t max_keys, int64_t window, int6
 }
 
 static Plan plan_simt(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t keys) {
-  return plan_split(S * Hkv * ((max_q * G + SR - 1) / SR), keys, 4 * 148, 128);
+  const int64_t SR = S_WARPS * simt_rows(S, Hkv, max_q * G);
+  return plan_split(S * Hkv * ((max_q * G + SR - 1) / SR), keys, 8 * 148, 128);
 }
 
 // Pairs up to which the few-rows kernel is taken where it serves the call: one
@@ -511,5 +576,5 @@ extern "C" int lsb_paged_attn(const void* q, const void* k_cache, const void* v_
   }
   const int rc = launch_simt(p, dtype, fp8, st);
   if (rc != LSB_OK || p.P == 1) return rc;
-  return launch_combine(p, SR, STK, dtype, st);
+  return launch_combine(p, S_WARPS * simt_rows(num_seqs, Hkv, max_seqlen_q * p.G), STK, dtype, st);
 }

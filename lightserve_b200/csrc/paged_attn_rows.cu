@@ -3,10 +3,13 @@
 //
 // One CTA: a query tile of 8 NH pairs (row, head of the group) of one
 // (sequence, cache head) and one chunk of its keys; its 4 warps take groups of
-// 16 keys in turn and merge at the end. Bound by HBM and, for e4m3, close to it
-// by instruction issue: per 16 keys a warp moves 4 KiB (D = 128) and issues 16
-// m16n8k16 MMAs per 8 pairs. The warp-level MMA is the right size here:
-// tcgen05's 128-row tiles would hold one row of use per key read.
+// 16 keys (e4m3: 32) in turn and merge at the end. Bound by HBM for a 16-bit
+// cache; over e4m3 by latency (65% of the DRAM rate, 43% of the issue slots, 12
+// warps an SM at 151 registers): half the bytes a key, the same number of MMAs,
+// 16 m16n8k16 per 16 keys and 8 pairs. The warp-level MMA is the right size
+// here: tcgen05's 128-row tiles would hold one row of use per key read.
+// Measured: 64 sequences, 16 heads of 128, 512-4096 keys, e4m3 114 us (5.2 TB/s);
+// 4096 keys each, 16-bit, 312 us (6.9 TB/s with what L2 keeps), e4m3 196 (5.5).
 //
 // Both products keep the cache on the MMA's 16-row side and the pairs on its
 // 8-column side, so a single query head wastes 7 of 8 columns and nothing else:
@@ -127,7 +130,9 @@ struct Shape {
   static constexpr int CPR = D * EB / 16;          // 16-byte pieces of a row: 4, 8 or 16
   static constexpr int TILE = TK * CPR * 16;       // bytes of a group's K (and V)
   static constexpr int STAGE = 2 * TILE;
-  // Groups in flight per warp, sized so that an SM holds about 190 KB of ring.
+  // Groups in flight per warp and CTAs per SM (registers): 96 to 196 KB of ring
+  // an SM. e4m3, D 64, one block of pairs: 5 CTAs 78 us, 3 CTAs 86 (64 sequences,
+  // 16 heads, 512-4096 keys).
   static constexpr int STAGES = FP8 ? 2 : (D == 64 ? 4 : 3);
   static constexpr int ctas(int nh) {
     return FP8 ? (D == 64 ? (nh == 1 ? 5 : 3) : (nh == 3 ? 2 : 3)) : (D == 64 ? 3 : 2);

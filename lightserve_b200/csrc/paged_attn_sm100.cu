@@ -23,8 +23,19 @@
 //  * A pair's heads of one group share the K/V tiles: row r of a tile is
 //    token r / G, head r % G.
 //
-// Warps: 0 loads (Q; K, V of a 16-bit cache), 1 issues MMAs and owns TMEM,
-// 4-7 and 8-11 softmax of query tile 0 and 1, 12-15 convert (e4m3 only).
+// What bounds it, per step of 128 keys at D = 128: the softmax's exponentials
+// (2 x 128 x 128 at 16 a clock, 2048 clocks) and the MMAs (2100 clocks at the
+// dense rate), overlapped but for the chain S -> P -> PV -> next S: about 3000
+// clocks, 61% of the tensor pipe and 62% of the exponential unit busy. At D = 64
+// the MMAs halve and the step stays. An e4m3 step is 27% longer: the converters
+// share shared memory and issue slots with the rest. Measured, 16 heads, one chunk
+// of 8192 tokens: D 128 bf16 222 us (1240 TFLOP/s), over e4m3 281; D 64 209 and 229.
+// (Tried: a share of the exponentials on the FMA pipe, +2 to +7%; an MMA warp per
+// query tile, +25%, the tiles fall into step; three S buffers at D = 64, +8%;
+// six converter warps, +3 to +11%.)
+//
+// Warps: 0 loads (Q; K, V of a 16-bit cache, raw tiles of an e4m3 one), 1 issues
+// MMAs and owns TMEM, 4-7 and 8-11 softmax of query tile 0 and 1, 12-15 convert (e4m3 only).
 // TMEM: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512) columns. Every
 // mbarrier wait is bounded; on a timeout the error word is set, the role ends,
 // TMEM is freed and the CTA exits.
