@@ -19,12 +19,14 @@ namespace pa {
 // are broadcast reads. P V: lane = dim, each V element serving the warp's pairs.
 // All arithmetic is fp32, as the fp32 model's parity with the reference needs
 // (tensor-core TF32 does not reach it).
-// ROWS = 1 serves up to 4 pairs (a tile of 16 took 197 us against 91 for 4
-// sequences of 2000-9000 fp32 keys, 8 cache heads of 128, 4 pairs: 38% of HBM);
-// 8, where half the CTAs still fill the GPU: shared-memory reads, 4 + ROWS
-// wavefronts per 4 ROWS FMAs of a warp, and issue slots bound it (4 chunks of
-// 300-700 tokens over 1000-4000, 8 x 2 heads of 128: 1650 us, 19 TFLOP/s, against
-// 2010 with 4; three short prompts 19 against 13).
+// ROWS = 1 serves up to 4 pairs (a tile of 16 took 197 us against 87 for 4
+// sequences of 2000-9000 fp32 keys, 8 cache heads of 128, 4 pairs: 39% of HBM), and
+// a single pair is shared by the warps (32 sequences of 512-4096 fp32 keys, 8
+// heads of 128, a window of 2048: 158 us against 126, 55% of HBM). ROWS = 8 where
+// half the CTAs still fill the GPU: shared-memory reads, 4 + ROWS wavefronts per
+// 4 ROWS FMAs of a warp, and issue slots bound it (4 chunks of 300-700 tokens over
+// 1000-4000, 8 x 2 heads of 128: 1610 us, 19 TFLOP/s, against 2010 with 4; three
+// short prompts 19 against 13).
 constexpr int STK = 32;
 constexpr int S_WARPS = 4;
 static int simt_rows(int64_t S, int64_t Hkv, int64_t pairs) {
@@ -32,37 +34,56 @@ static int simt_rows(int64_t S, int64_t Hkv, int64_t pairs) {
   return pairs > 16 && S * Hkv * ((pairs + 31) / 32) >= 2 * 148 ? 8 : 4;
 }
 
-// Four elements of a cached row as they are stored; `left` of them exist.
+// Four elements of a cached row as they are stored, in whole words: unpacking
+// them where they are loaded waited for each load in turn (64 sequences of
+// 512-4096 e4m3 keys, 16 heads of 128, fp32 q: 1995 us against 586).
 template <typename KV>
 struct alignas(4 * sizeof(KV)) Quad {
-  KV e[4];
+  uint32_t w[sizeof(KV)];
 };
 
+// `left` of the elements exist.
 template <typename KV>
 __device__ __forceinline__ Quad<KV> load4(const KV* p, bool vec, int left) {
   if (vec) return *reinterpret_cast<const Quad<KV>*>(p);
   Quad<KV> x = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < left) x.e[i] = p[i];
+  for (int i = 0; i < 4; ++i) {
+    if (i >= left) break;
+    if constexpr (sizeof(KV) == 1)
+      x.w[0] |= (uint32_t)reinterpret_cast<const uint8_t*>(p)[i] << (8 * i);
+    else if constexpr (sizeof(KV) == 2)
+      x.w[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i % 2));
+    else
+      x.w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
   return x;
 }
 
-__device__ __forceinline__ float4 widen(const Quad<uint8_t>& x) {
-  float f[4];
-  e4m3x4_to_float(*reinterpret_cast<const uint32_t*>(x.e), f);
-  return make_float4(f[0], f[1], f[2], f[3]);
-}
 template <typename KV>
 __device__ __forceinline__ float4 widen(const Quad<KV>& x) {
-  return make_float4(to_f(x.e[0]), to_f(x.e[1]), to_f(x.e[2]), to_f(x.e[3]));
+  if constexpr (sizeof(KV) == 1) {
+    float f[4];
+    e4m3x4_to_float(x.w[0], f);
+    return make_float4(f[0], f[1], f[2], f[3]);
+  } else if constexpr (sizeof(KV) == 2) {
+    KV e[4];
+    memcpy(e, x.w, sizeof(e));
+    return make_float4(to_f(e[0]), to_f(e[1]), to_f(e[2]), to_f(e[3]));
+  } else {
+    return make_float4(__uint_as_float(x.w[0]), __uint_as_float(x.w[1]), __uint_as_float(x.w[2]),
+                       __uint_as_float(x.w[3]));
+  }
 }
 
-// DC: 32-dim columns per lane (head dim up to 32 DC).
-template <typename T, typename KV, int DC, int ROWS>
+// DC: 32-dim columns per lane (head dim up to 32 DC). ONE: the call has one pair per
+// cache head, which the warps share: a quarter of the dims of each score, then a
+// quarter of the keys of P V.
+template <typename T, typename KV, int DC, int ROWS, bool ONE>
 __global__ void __launch_bounds__(S_WARPS * 32)
 paged_simt_kernel(const Params p, const bool vec) {
   constexpr bool FP8 = std::is_same<KV, uint8_t>::value;
+  static_assert(!ONE || ROWS == 1, "one pair");
   constexpr int SR = S_WARPS * ROWS;
   // Staging: a warp's 8 keys of a tile, QL lanes per key, QPL quads per lane.
   constexpr int QL = DC == 2 ? 16 : 32, QPL = DC == 8 ? 2 : 1;
@@ -102,10 +123,10 @@ paged_simt_kernel(const Params p, const bool vec) {
   int pos[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
-    const int pr = tile * SR + r * S_WARPS + warp;
+    const int pr = ONE ? 0 : tile * SR + r * S_WARPS + warp;
     pos[r] = pr < pairs ? q.pos0 + pr / p.G : -1;  // position -1 sees nothing
   }
-  const bool live = tile * SR + warp < pairs;
+  const bool live = ONE || tile * SR + warp < pairs;
   float m[ROWS], l[ROWS], acc[ROWS][DC];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
@@ -190,16 +211,21 @@ paged_simt_kernel(const Params p, const bool vec) {
     if (!live) continue;
     float sc[ROWS] = {};
 #pragma unroll 2
-    for (int d = 0; d < Dp; d += 4) {
+    for (int d = ONE ? 4 * warp : 0; d < Dp; d += ONE ? 4 * S_WARPS : 4) {
       const float4 kx = *reinterpret_cast<const float4*>(sK + lane * ldk + d);
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        const float4 qx = *reinterpret_cast<const float4*>(sQ + (r * S_WARPS + warp) * Dp + d);
+        const float4 qx = *reinterpret_cast<const float4*>(sQ + (ONE ? 0 : r * S_WARPS + warp) * Dp + d);
         sc[r] = fmaf(qx.x, kx.x, sc[r]);
         sc[r] = fmaf(qx.y, kx.y, sc[r]);
         sc[r] = fmaf(qx.z, kx.z, sc[r]);
         sc[r] = fmaf(qx.w, kx.w, sc[r]);
       }
+    }
+    if constexpr (ONE) {
+      sP[warp * STK + lane] = sc[0];
+      __syncthreads();
+      sc[0] = (sP[lane] + sP[STK + lane]) + (sP[2 * STK + lane] + sP[3 * STK + lane]);
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
@@ -213,8 +239,20 @@ paged_simt_kernel(const Params p, const bool vec) {
       l[r] = l[r] * a + e;  // per-lane partial sum
 #pragma unroll
       for (int c = 0; c < DC; ++c) acc[r][c] *= a;
-      sP[(warp * ROWS + r) * STK + lane] = e;
+      if constexpr (ONE) {
+        const float* vt = sV + warp * (STK / S_WARPS) * Dp;
+#pragma unroll
+        for (int j = 0; j < STK / S_WARPS; ++j) {
+          const float pe = __shfl_sync(0xffffffffu, e, warp * (STK / S_WARPS) + j);
+#pragma unroll
+          for (int c = 0; c < DC; ++c)
+            if (c * 32 + lane < Dp) acc[r][c] = fmaf(pe, vt[j * Dp + c * 32 + lane], acc[r][c]);
+        }
+      } else {
+        sP[(warp * ROWS + r) * STK + lane] = e;
+      }
     }
+    if constexpr (ONE) continue;
     __syncwarp();
     for (int j = 0; j < STK; j += 4) {
       float4 pr[ROWS];
@@ -235,6 +273,17 @@ paged_simt_kernel(const Params p, const bool vec) {
         }
       }
     }
+  }
+  if constexpr (ONE) {  // the warps' shares of P V (every warp has the statistics)
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < DC; ++c) sK[warp * (DC * 32) + c * 32 + lane] = acc[0][c];
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int w = 1; w < S_WARPS; ++w) acc[0][c] += sK[w * (DC * 32) + c * 32 + lane];
   }
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
@@ -268,7 +317,7 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
   LSB_CHECK_ARG(tiles <= 65535 && (int64_t)p.Hkv * p.P <= 0x7fffffff,
                 "paged_attn: %lld query tiles per head exceed 65535 (CUDA-core kernel)", (long long)tiles);
   const dim3 grid((unsigned)(p.Hkv * p.P), (unsigned)tiles, (unsigned)p.S);
-  auto go = [&](auto tag, auto kvtag, auto dc, auto nr) -> int {
+  auto go = [&](auto tag, auto kvtag, auto dc, auto nr, auto one) -> int {
     using T = decltype(tag);
     using KV = decltype(kvtag);
     constexpr int DC = decltype(dc)::value;
@@ -276,7 +325,7 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
     const bool vec = p.D % 4 == 0 &&
                      ((reinterpret_cast<uintptr_t>(p.k_cache) | reinterpret_cast<uintptr_t>(p.v_cache)) &
                       (4 * sizeof(KV) - 1)) == 0;
-    auto kern = paged_simt_kernel<T, KV, DC, decltype(nr)::value>;
+    auto kern = paged_simt_kernel<T, KV, DC, decltype(nr)::value, decltype(one)::value>;
     static SmemLimit limit;
     if (smem > 48 * 1024)
       if (int rc = limit.ensure(kern, smem, "paged_attn smem attribute")) return rc;
@@ -285,9 +334,11 @@ int launch_simt(const Params& p, int dtype, bool kv_fp8, cudaStream_t st) {
     return LSB_OK;
   };
   auto by_rows = [&](auto tag, auto kvtag, auto dc) -> int {
-    if (rows == 1) return go(tag, kvtag, dc, std::integral_constant<int, 1>{});
-    if (rows == 4) return go(tag, kvtag, dc, std::integral_constant<int, 4>{});
-    return go(tag, kvtag, dc, std::integral_constant<int, 8>{});
+    using std::integral_constant;
+    if ((int64_t)p.max_q * p.G == 1) return go(tag, kvtag, dc, integral_constant<int, 1>{}, std::true_type{});
+    if (rows == 1) return go(tag, kvtag, dc, integral_constant<int, 1>{}, std::false_type{});
+    if (rows == 4) return go(tag, kvtag, dc, integral_constant<int, 4>{}, std::false_type{});
+    return go(tag, kvtag, dc, integral_constant<int, 8>{}, std::false_type{});
   };
   auto by_dim = [&](auto tag, auto kvtag) -> int {
     if (p.D <= 64) return by_rows(tag, kvtag, std::integral_constant<int, 2>{});
