@@ -459,11 +459,11 @@ static Plan plan_simt(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t 
 }
 
 // Pairs up to which the few-rows kernel is taken where it serves the call: one
-// of its tiles. Measured with both kernels, bf16: 32 sequences of 512-4096
-// keys, 8 cache heads of 128, 20 pairs: 84 us against the tcgen05 kernel's 105
-// (1000-2000 keys, 16 / 24 / 32 pairs: 60 / 74 / 106 against 62); 16 heads of
-// 64: 24 / 32 pairs 88 / 131 against 98; one sequence of 16000 keys, 8 heads of
-// 128: 16 / 24 / 32 pairs 21.0 / 24 / 33 against 21; e4m3 alike.
+// of its tiles. Measured against the tcgen05 kernel, bf16, 8 cache heads of 128 and 4
+// query heads each: 32 sequences of 512-4096 keys with 1-5 / 5 / 6 new tokens 82 /
+// 91 / 95 us against 94 / 90 / 91, over e4m3 91 / 101 / 106 against 120; 16 heads of
+// 64, 20 pairs 110 against 127; above, 32 pairs 90 against 74. One sequence would
+// cross at 16 pairs (16000 keys: 17 / 23 us at 16 / 24 pairs against 20).
 constexpr int64_t ROWS_MAX_PAIRS = 24;
 
 // The few-rows kernel's chunks: as many as give 3 CTAs per SM, of at most 1024
