@@ -26,7 +26,7 @@
 // What bounds it, per step of 128 keys at D = 128: the softmax's exponentials
 // (2 x 128 x 128 at 16 a clock, 2048 clocks) and the MMAs (2100 clocks at the
 // dense rate), overlapped but for the chain S -> P -> PV -> next S: about 3000
-// clocks, 61% of the tensor pipe and 62% of the exponential unit busy. At D = 64
+// clocks, 65% of the tensor pipe and 65% of the exponential unit busy. At D = 64
 // the MMAs halve and the step stays. An e4m3 step is 27% longer: the converters
 // share shared memory and issue slots with the rest. Measured, 16 heads, one chunk
 // of 8192 tokens: D 128 bf16 222 us (1240 TFLOP/s), over e4m3 281; D 64 209 and 229.
