@@ -111,6 +111,25 @@ def test_other_head_dims(D, dtype, quantised):
     _check(R.build([70, 40], [20, 1], 2, 2, D, 16, dtype, quantised=quantised, seed=D))
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 9)])
+@pytest.mark.parametrize("dtype,D,G,quantised", [(F32, 64, 1, False), (F32, 128, 2, True), (BF16, 96, 1, False),
+                                                 (F16, 200, 2, True), (F32, 33, 1, False)])
+def test_many_rows_on_the_cuda_cores(dtype, D, G, quantised, window, sinks):
+    """Enough query tiles to fill the GPU: 8 pairs a warp."""
+    b = R.build([640, 700], [640 // G, 601 // G], 8, G, D, 16, dtype, quantised=quantised, seed=23)
+    _check(b, window, sinks, _lib.IMPL_SIMT)
+
+
+@pytest.mark.parametrize("lens", [[1], [31, 32, 33], [700, 5, 0, 2100]])
+@pytest.mark.parametrize("dtype,D,quantised", [(F32, 64, False), (F32, 128, True), (BF16, 96, True), (F16, 250, False),
+                                               (F32, 1, False), (BF16, 20, True)])
+@pytest.mark.parametrize("window", [None, 40])
+def test_one_pair_on_the_cuda_cores(lens, dtype, D, quantised, window):
+    """Plain decode there: the warps share one pair."""
+    b = R.build(lens, [1] * len(lens), 3, 1, D, 8, dtype, quantised=quantised, seed=24)
+    _check(b, window, 2 if window else 0, _lib.IMPL_SIMT)
+
+
 @pytest.mark.parametrize("quantised", [False, True])
 @pytest.mark.parametrize("window,sinks", [(None, 0), (90, 20)])
 @pytest.mark.parametrize("new", [[1, 1, 1], [4, 2, 5], [200, 1, 129]])
