@@ -27,9 +27,9 @@
 // (2 x 128 x 128 at 16 a clock, 2048 clocks) and the MMAs (2100 clocks at the
 // dense rate), overlapped but for the chain S -> P -> PV -> next S: about 3000
 // clocks, 65% of the tensor pipe and 65% of the exponential unit busy. At D = 64
-// the MMAs halve and the step stays. An e4m3 step is 27% longer: the converters
+// the MMAs halve and the step stays. An e4m3 step is 22% longer: the converters
 // share shared memory and issue slots with the rest. Measured, 16 heads, one chunk
-// of 8192 tokens: D 128 bf16 222 us (1240 TFLOP/s), over e4m3 281; D 64 209 and 229.
+// of 8192 tokens: D 128 bf16 222 us (1240 TFLOP/s), over e4m3 272; D 64 209 and 228.
 // (Tried: a share of the exponentials on the FMA pipe, +2 to +7%; an MMA warp per
 // query tile, +25%, the tiles fall into step; three S buffers at D = 64, +8%;
 // six converter warps, +3 to +11%.)
@@ -124,6 +124,17 @@ __device__ __forceinline__ uint32_t desc_lo(const void* p, int lbo) {
   return (smem_u32(p) >> 4) | (uint32_t)(lbo >> 4) << 16;
 }
 constexpr uint32_t desc_hi(int sbo) { return (uint32_t)(sbo >> 4) | 1u << 14 | 2u << 29; }
+
+// Two fp16 values times an fp16 factor, in fp32 (exact), without widening them
+// first (bf16 over e4m3, one chunk of 8192 tokens, D 128: 281 us against 272).
+__device__ __forceinline__ float2 mul_widen(uint32_t z, uint16_t f) {
+  float2 y;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "fma.rn.f32.f16 %0, l, %3, %4;\n\tfma.rn.f32.f16 %1, h, %3, %4;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "r"(z), "h"(f), "f"(-0.f));
+  return y;
+}
 
 template <int N>
 __device__ __forceinline__ float row_max(const uint32_t (&sr)[N][32]) {
@@ -607,17 +618,25 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       constexpr int RPP = 128 / CPR;        // rows per pass of the 128 threads
       constexpr int PASSES = BN / RPP;
       const int tid = threadIdx.x & 127, c = tid % CPR, r0 = tid / CPR;
-      auto store = [&](int i, const uint4& raw16, int scale, bool plain, uint8_t* tile) {
+      auto store = [&](int i, const uint4& raw16, int scale, auto plain, uint8_t* tile) {
         const int kc = c / 4, row = r0 + i * RPP;
         const uint32_t words[4] = {raw16.x, raw16.y, raw16.z, raw16.w};
         uint32_t o[8];
-        if (FMT == 0 && plain) {  // the scale is an fp16 and no product leaves fp16's range
+        // plain: the scale is an fp16, and no product leaves fp16's range.
+        if constexpr (FMT == 0 && decltype(plain)::value) {
           const __half2 f = __half2half2(__float2half_rn(e8m0_to_float(scale)));
 #pragma unroll
           for (int i2 = 0; i2 < 8; ++i2) {
             const uint32_t z = cvt_e4m3x2_f16x2((uint16_t)(words[i2 / 2] >> (16 * (i2 & 1))));
             const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&z), f);
             o[i2] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+        } else if constexpr (decltype(plain)::value) {
+          const uint16_t f = __half_as_ushort(__float2half_rn(e8m0_to_float(scale)));
+#pragma unroll
+          for (int i2 = 0; i2 < 8; ++i2) {
+            const float2 y = mul_widen(cvt_e4m3x2_f16x2((uint16_t)(words[i2 / 2] >> (16 * (i2 & 1)))), f);
+            o[i2] = pack_bf16(y.x, y.y);
           }
         } else {
           const float f = e8m0_to_float(scale);
@@ -673,13 +692,20 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             ok = false;
             break;
           }
-          // fp16: every scale between 2^-24 and 2^7 (448 2^7 is below 65504).
+          // Every scale between 2^-24 and 2^7 (448 2^7 is below 65504).
           bool plain = true;
 #pragma unroll
           for (int i = 0; i < PASSES; ++i) plain = plain && e[i] >= 103 && e[i] <= 134;
-          if (FMT == 0) plain = __all_sync(0xffffffffu, plain);
+          plain = __all_sync(0xffffffffu, plain);
+          // One branch for the tile: a branch per pass kept the passes apart (fp16 over
+          // e4m3, one chunk of 8192 tokens, D 128: 288 us against 252).
+          if (plain) {
 #pragma unroll
-          for (int i = 0; i < PASSES; ++i) store(i, x[i], e[i], plain, tile);
+            for (int i = 0; i < PASSES; ++i) store(i, x[i], e[i], std::true_type{}, tile);
+          } else {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) store(i, x[i], e[i], std::false_type{}, tile);
+          }
           fence_async_shared();
           __syncwarp();
           // The raw tile is released once its values have been used: an arrival does
