@@ -27,9 +27,9 @@
 // (2 x 128 x 128 at 16 a clock, 2048 clocks) and the MMAs (2100 clocks at the
 // dense rate), overlapped but for the chain S -> P -> PV -> next S: about 3000
 // clocks, 65% of the tensor pipe and 65% of the exponential unit busy. At D = 64
-// the MMAs halve and the step stays. An e4m3 step is 22% longer: the converters
+// the MMAs halve and the step stays. An e4m3 step is 17% longer: the converters
 // share shared memory and issue slots with the rest. Measured, 16 heads, one chunk
-// of 8192 tokens: D 128 bf16 222 us (1240 TFLOP/s), over e4m3 272; D 64 209 and 228.
+// of 8192 tokens: D 128 bf16 222 us (1240 TFLOP/s), over e4m3 259; D 64 209 and 232.
 // (Tried: a share of the exponentials on the FMA pipe, +2 to +7%; an MMA warp per
 // query tile, +25%, the tiles fall into step; three S buffers at D = 64, +8%;
 // six converter warps, +3 to +11%.)
@@ -622,9 +622,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         const int kc = c / 4, row = r0 + i * RPP;
         const uint32_t words[4] = {raw16.x, raw16.y, raw16.z, raw16.w};
         uint32_t o[8];
-        // plain: the scale is an fp16, and no product leaves fp16's range.
+        // plain: the scale is an fp16, and no product leaves fp16's range (nor is its
+        // byte one of e8m0's special ones).
         if constexpr (FMT == 0 && decltype(plain)::value) {
-          const __half2 f = __half2half2(__float2half_rn(e8m0_to_float(scale)));
+          const __half2 f = __half2half2(__float2half_rn(__uint_as_float((uint32_t)scale << 23)));
 #pragma unroll
           for (int i2 = 0; i2 < 8; ++i2) {
             const uint32_t z = cvt_e4m3x2_f16x2((uint16_t)(words[i2 / 2] >> (16 * (i2 & 1))));
@@ -632,7 +633,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             o[i2] = *reinterpret_cast<const uint32_t*>(&y);
           }
         } else if constexpr (decltype(plain)::value) {
-          const uint16_t f = __half_as_ushort(__float2half_rn(e8m0_to_float(scale)));
+          const uint16_t f = __half_as_ushort(__float2half_rn(__uint_as_float((uint32_t)scale << 23)));
 #pragma unroll
           for (int i2 = 0; i2 < 8; ++i2) {
             const float2 y = mul_widen(cvt_e4m3x2_f16x2((uint16_t)(words[i2 / 2] >> (16 * (i2 & 1)))), f);
