@@ -57,17 +57,19 @@ constexpr int WARPS = 4;
 constexpr float RAISE = 8.f;   // log2: how far a score may exceed the reference maximum
 constexpr float LIFT = 7.f;    // log2: factor on every weight
 
+// (volatile: a group's MMAs, and with them the uses of its loads, stay ahead of
+// the next group's wait and copies.)
 template <bool F16>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (F16)
-    asm(
+    asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm(
+    asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -560,8 +562,11 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
         sm100::mbar_wait_warp(&full[i % S::STAGES], (i / S::STAGES) & 1, 0x601);
       break;
     }
-    // (Group n - 1 has been read by all lanes: its loads fed MMAs before the
-    // vote above.)
+    // The next boxes go where group n - 1 was, by another proxy than the one
+    // that read (and, at a span's ends, zeroed) it. The reads are plain loads, for
+    // which a vote does not wait: each lane's fence orders them before the boxes,
+    // which the warp issues behind a __syncwarp. (No cost measured.)
+    sm100::fence_async_shared();
     there |= copy_next(n + AHEAD) << (S::GR * AHEAD);
     uint8_t* st = ring + (n % S::STAGES) * S::STAGE;
     if (!all_seen(tok0)) {
@@ -571,7 +576,6 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
       if (!seen_by_any(p, pos_lo, pos_hi, q.ctx, tok0 + k))
         for (int c = lane / TK; c < S::CPR; c += 32 / TK)
           *reinterpret_cast<uint4*>(st + S::TILE + S::at(k, c)) = make_uint4(0u, 0u, 0u, 0u);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next boxes
       __syncwarp();
     }
     float sc[NH][NU][4];

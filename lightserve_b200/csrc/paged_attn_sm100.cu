@@ -94,10 +94,6 @@ __device__ __forceinline__ void st_global_v8(void* dst, const uint32_t* w) {
                : "memory");
 }
 
-__device__ __forceinline__ void fence_async_shared() {
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-
 // The n lowest bits set (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t low_bits(int n) {
   return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u;

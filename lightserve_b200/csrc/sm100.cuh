@@ -99,6 +99,12 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
 }
 
 // ------------------------------------------------------------------ TMA ---
+// Orders this thread's ordinary shared-memory reads and writes before the
+// async proxy's (TMA copies, tcgen05 operands) that follow it.
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
                                             int c0, int c1, int c2, int c3) {
   asm volatile(
