@@ -582,7 +582,11 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           uint32_t pk[16];
 #pragma unroll
           for (int cc = 0; cc < 16; ++cc) {
-            const float a0 = __uint_as_float(ov[2 * cc]), a1 = __uint_as_float(ov[2 * cc + 1]);
+            float a0 = __uint_as_float(ov[2 * cc]), a1 = __uint_as_float(ov[2 * cc + 1]);
+            if constexpr (FP8) {  // P's rounding can lift O past T's largest value
+              a0 = clamp_finite<T>(a0);
+              a1 = clamp_finite<T>(a1);
+            }
             pk[cc] = FMT == 1 ? pack_bf16(a0, a1) : pack_f16(a0, a1);
           }
           if (st32) {
