@@ -62,6 +62,11 @@ constexpr int CHUNK_BYTES = 128 * 128;  // Q: [128 rows][64 columns] of 16 bits
 // TMA box over [cache rows / 8, D / 64, 8, 64] delivers a whole page.
 constexpr int ATOM = 1024;
 constexpr float RESCALE_THRESHOLD = 8.0f;
+// log2 of a factor on every weight of an fp16 P: 2^15 at most with the threshold,
+// and full precision down to 2^-21 of the running maximum instead of 2^-14, nothing
+// below 2^-32 instead of 2^-25 (a key that takes nearly all the weight beside
+// tens of thousands of small ones: they are still summed). bf16 has fp32's range.
+constexpr float F16_LIFT = 7.0f;
 
 template <int D, bool FP8>
 struct Smem {
@@ -456,6 +461,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const int row = threadIdx.x - 128 * (t + 1);  // TMEM lane
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float sl2 = p.scale_log2;
+    constexpr float LIFT = FMT == 0 ? F16_LIFT : 0.f;
     const int nkv_t = t == 0 ? w.nkv_t[0] : w.nkv_t[1];
     const int pr = (w.c0 + t) * w.R + row;
     const bool mine = row < w.R && pr < w.pairs;
@@ -515,7 +521,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       const float m_use = (m == -INFINITY) ? 0.f : m;
       float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                       make_float2(0.f, 0.f)};
-      const float2 sl2_2 = make_float2(sl2, sl2), negm2 = make_float2(-m_use, -m_use);
+      const float2 sl2_2 = make_float2(sl2, sl2), negm2 = make_float2(LIFT - m_use, LIFT - m_use);
       auto weigh = [&](const uint32_t (&x)[32], uint32_t* pk) {  // 32 scores to 16 packed pairs
 #pragma unroll
         for (int cc = 0; cc < 16; ++cc) {
@@ -602,7 +608,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         __syncwarp();
       }
       if (mine) {
-        const float lse2 = none ? -INFINITY : m + log2f(l);
+        const float lse2 = none ? -INFINITY : m + log2f(l) - LIFT;
         if (w.chunks > 1)
           p.part_lse[at] = lse2;
         else if (p.lse != nullptr)

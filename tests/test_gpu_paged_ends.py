@@ -68,3 +68,46 @@ def test_fp16_results_over_e4m3_stay_at_the_largest_value(raised, new, D, impl):
     o, tol, _, _ = _want(b, scale)
     assert abs(float(o.min()) - 65536.0) < 1e-6  # what e4m3 makes of 65504
     R.check(out, o.clamp(max=65504.0), tol + 32)
+
+
+@pytest.mark.parametrize("impl", IMPLS)
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("below", [24.6, 25.5])
+@pytest.mark.parametrize("sink", [3, 24000])
+def test_many_small_weights_beside_a_large_one(sink, below, D, quantised, impl):
+    """One key that takes nearly all the weight and holds V = 0 (an attention sink), and the 24576 to 32767 others a
+    row sees `below` powers of two under it with V = 1: together they are the result. As many rows as keep a key range
+    whole (ranges are joined in fp32).
+
+    In fp16 the weights carry 2^7 and are off by at most half of its smallest step: 2^-25 beside a sum of 2^7 or more,
+    2^-32 of each |v|. The other terms are those of ``paged_reference``."""
+    n, new, G, bs = 32768, 8192, 4, 16
+    g = torch.Generator().manual_seed(62)
+    table = torch.randperm(n // bs, generator=g)
+    at = table[torch.arange(n) // bs], 0, torch.arange(n) % bs
+    k, v = (torch.zeros(n // bs, 1, bs, D, dtype=F16) for _ in range(2))
+    k[(*at, 0)] = -1.0
+    v[at] = 1.0
+    k[table[sink // bs], 0, sink % bs], v[table[sink // bs], 0, sink % bs] = 0.0, 0.0
+    ks = vs = None
+    if quantised:
+        (k, ks), (v, vs) = ((q.float().to(torch.float8_e4m3fn).cuda(), e.float().to(torch.float8_e8m0fnu).cuda())
+                            for q, e in (R.quantise(k), R.quantise(v)))
+    q = torch.zeros(new, G, D, dtype=F16)
+    q[..., 0] = 1
+    lse = torch.empty(G, new, device="cuda")
+    scale = below * math.log(2)
+    out = _paged_attn(q.cuda(), k.cuda(), v.cuda(), table[None].to(torch.int32).cuda(),
+                      torch.tensor([n], dtype=torch.int32, device="cuda"),
+                      torch.tensor([0, new], dtype=torch.int32, device="cuda"), new, None, 0, ks, vs, scale, None, lse,
+                      None, IMPLS[impl])
+    others = torch.arange(n - new, n, dtype=torch.float64)  # keys a row sees beside the sink
+    w = 2.0 ** -below
+    o = others * w / (1 + others * w)
+    u, u32 = 2.0 ** -11, 2.0 ** -24
+    slack = 2 * (D + 4) * u32 * scale + 2.0 ** -21 + (n + 64) * u32
+    tol = (1 + 4 * u) * (2 * u + 2 * slack) * o + 2.0 ** -25 + 2.0 ** -32 * others
+    R.check(out, o[:, None, None].expand(out.shape), tol[:, None, None].expand(out.shape))
+    l = torch.log1p(others * w)
+    R.check(lse, l.expand(lse.shape), (slack + 2.0 ** -22 * (1 + l)).expand(lse.shape), "lse")
