@@ -28,6 +28,15 @@ namespace pa {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// The tensor-core kernels' running maximum may lag a score by 2^8 (it is raised,
+// and the outputs rescaled, only beyond that). An fp16 P also carries 2^7 on every
+// weight: 2^15 at most, and full precision down to 2^-21 of the running maximum
+// instead of 2^-14, nothing below 2^-32 instead of 2^-25 (a key that takes
+// nearly all the weight beside tens of thousands of small ones: they are still
+// summed). bf16 has fp32's range and carries nothing, so a sum passes fp32's
+// only where values times keys pass 2^120.
+constexpr float F16_LIFT = 7.f;
+
 struct Params {
   const void* q;
   const void* k_cache;

@@ -38,10 +38,9 @@
 // value; below that the error is under 2^-39 of it).
 //
 // The running maximum is raised only when a score exceeds it by 2^8 (a vote
-// per group instead of shuffles and a rescale). Weights carry a factor 2^7, so
-// an fp16 weight keeps its precision down to 2^-21 of the maximum and vanishes
-// below 2^-32: rounding P to 16 bits is off by half a step of the operand type
-// relative to each weight, as in the framework's other attention kernels.
+// per group instead of shuffles and a rescale). Weights of an fp16 P carry 2^7
+// (paged_attn.cuh): rounding P to 16 bits is off by half a step of the operand
+// type relative to each weight, as in the framework's other attention kernels.
 #include "paged_attn.cuh"
 #include "sm100.cuh"
 #include "tma_host.cuh"
@@ -55,7 +54,6 @@ namespace rows {
 
 constexpr int WARPS = 4;
 constexpr float RAISE = 8.f;   // log2: how far a score may exceed the reference maximum
-constexpr float LIFT = 7.f;    // log2: factor on every weight
 
 // (volatile: a group's MMAs, and with them the uses of its loads, stay ahead of
 // the next group's wait and copies.)
@@ -168,6 +166,7 @@ paged_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant_
   wait_prerequisites();
   using S = Shape<FP8, D>;
   constexpr bool F16 = FP8 || std::is_same<T, __half>::value;  // MMA operand type
+  constexpr float LIFT = F16 ? F16_LIFT : 0.f;                 // log2: factor on every weight
   // NE: of a lane's pairs 8 h + 2 t and + 1, those that can be in use (ONE: the
   // call has one pair per cache head, plain decode).
   constexpr int R = 8 * NH, TK = S::TK, NU = S::NU, NE = ONE ? 1 : 2;

@@ -62,11 +62,6 @@ constexpr int CHUNK_BYTES = 128 * 128;  // Q: [128 rows][64 columns] of 16 bits
 // TMA box over [cache rows / 8, D / 64, 8, 64] delivers a whole page.
 constexpr int ATOM = 1024;
 constexpr float RESCALE_THRESHOLD = 8.0f;
-// log2 of a factor on every weight of an fp16 P: 2^15 at most with the threshold,
-// and full precision down to 2^-21 of the running maximum instead of 2^-14, nothing
-// below 2^-32 instead of 2^-25 (a key that takes nearly all the weight beside
-// tens of thousands of small ones: they are still summed). bf16 has fp32's range.
-constexpr float F16_LIFT = 7.0f;
 
 template <int D, bool FP8>
 struct Smem {

@@ -10,7 +10,7 @@ from lightserve_b200.kernels.paged_chunk_attention import _paged_attn
 
 pytestmark = pytest.mark.gpu
 
-F16 = torch.float16
+BF16, F16 = torch.bfloat16, torch.float16
 IMPLS = {"auto": _lib.IMPL_AUTO, "simt": _lib.IMPL_SIMT, "rows": _lib.IMPL_ROWS, "tc": _lib.IMPL_TCGEN05}
 
 
@@ -111,3 +111,23 @@ def test_many_small_weights_beside_a_large_one(sink, below, D, quantised, impl):
     R.check(out, o[:, None, None].expand(out.shape), tol[:, None, None].expand(out.shape))
     l = torch.log1p(others * w)
     R.check(lse, l.expand(lse.shape), (slack + 2.0 ** -22 * (1 + l)).expand(lse.shape), "lse")
+
+
+@pytest.mark.parametrize("impl", IMPLS)
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+def test_large_values_in_bf16(new, D, quantised, impl):
+    """Values times the keys a row sees (32: two pages are there) just below 2^119, one key 7.9 powers of two above an
+    earlier one: its weight may stay at 2^7.9 (a running maximum is raised from 2^8 on)."""
+    keys = torch.full((240 + new,), HIDDEN)
+    keys[5], keys[192] = -1.0, 0.0
+    scale = 7.9 * math.log(2)
+    b = _scored(keys, torch.full_like(keys, 1.5 * 2.0 ** 113), new, D, BF16, quantised)
+    hidden = torch.ones_like(b["block_tables"], dtype=torch.bool)
+    hidden[0, [0, 12]] = False
+    b["block_tables"][hidden] = -1
+    out, _ = _run(b, scale, impl)
+    o, tol, _, _ = _want(b, scale)
+    assert 2.0 ** 118 < float(o.max()) * 32 < 2.0 ** 119
+    R.check(out, o, tol)
