@@ -74,8 +74,9 @@ __device__ __forceinline__ float finite_abs(float x) {
 __device__ __forceinline__ float scaled_for_e4m3(float x, float inv) { return fmaf(x, inv, x - x); }
 
 // Rounding to e4m3 can lift a value at the top of T's range past it (65504
-// becomes 65536): a dequantised row, and an attention output made of such
-// values, stays at T's largest finite value. NaN stays NaN.
+// becomes 65536): a dequantised row, and an fp16 attention output made of such
+// values, stays at T's largest finite value (a wider type's values of that size
+// are past what attention's fp32 sums hold). NaN stays NaN.
 template <typename T> struct FiniteMax;
 template <> struct FiniteMax<float> { static constexpr float v = 3.402823466e38f; };
 template <> struct FiniteMax<__nv_bfloat16> { static constexpr float v = 3.38953139e38f; };

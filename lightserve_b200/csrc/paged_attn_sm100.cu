@@ -456,7 +456,6 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     const int row = threadIdx.x - 128 * (t + 1);  // TMEM lane
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float sl2 = p.scale_log2;
-    constexpr float LIFT = FMT == 0 ? F16_LIFT : 0.f;
     const int nkv_t = t == 0 ? w.nkv_t[0] : w.nkv_t[1];
     const int pr = (w.c0 + t) * w.R + row;
     const bool mine = row < w.R && pr < w.pairs;
@@ -514,9 +513,10 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         l *= alpha;
       }
       const float m_use = (m == -INFINITY) ? 0.f : m;
+      const float neg_m = FMT == 0 ? F16_LIFT - m_use : -m_use;
       float2 l2[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                       make_float2(0.f, 0.f)};
-      const float2 sl2_2 = make_float2(sl2, sl2), negm2 = make_float2(LIFT - m_use, LIFT - m_use);
+      const float2 sl2_2 = make_float2(sl2, sl2), negm2 = make_float2(neg_m, neg_m);
       auto weigh = [&](const uint32_t (&x)[32], uint32_t* pk) {  // 32 scores to 16 packed pairs
 #pragma unroll
         for (int cc = 0; cc < 16; ++cc) {
@@ -584,7 +584,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 #pragma unroll
           for (int cc = 0; cc < 16; ++cc) {
             float a0 = __uint_as_float(ov[2 * cc]), a1 = __uint_as_float(ov[2 * cc + 1]);
-            if constexpr (FP8) {  // P's rounding can lift O past T's largest value
+            if constexpr (FP8 && FMT == 0) {  // P's rounding can lift O past fp16's largest value
               a0 = clamp_finite<T>(a0);
               a1 = clamp_finite<T>(a1);
             }
@@ -603,7 +603,7 @@ paged_chunk_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         __syncwarp();
       }
       if (mine) {
-        const float lse2 = none ? -INFINITY : m + log2f(l) - LIFT;
+        const float lse2 = none ? -INFINITY : m + log2f(l) - (FMT == 0 ? F16_LIFT : 0.f);
         if (w.chunks > 1)
           p.part_lse[at] = lse2;
         else if (p.lse != nullptr)
