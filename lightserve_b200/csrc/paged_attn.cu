@@ -463,7 +463,10 @@ static Plan plan_simt(int64_t S, int64_t max_q, int64_t Hkv, int64_t G, int64_t 
 // query heads each: 32 sequences of 512-4096 keys with 1-5 / 5 / 6 new tokens 82 /
 // 91 / 95 us against 94 / 90 / 91, over e4m3 91 / 101 / 106 against 120; 16 heads of
 // 64, 20 pairs 110 against 127; above, 32 pairs 90 against 74. One sequence would
-// cross at 16 pairs (16000 keys: 17 / 23 us at 16 / 24 pairs against 20).
+// cross at 16 pairs (16000 keys: 17 / 23 us at 16 / 24 pairs against 20). So one
+// bound for both caches and all batches gives up 1 to 4% over a 16-bit cache where
+// every sequence brings 20 to 24 pairs, and 15% for one sequence, for the 11 to
+// 24% that ragged batches and e4m3 gain.
 constexpr int64_t ROWS_MAX_PAIRS = 24;
 
 // The few-rows kernel's chunks: as many as give 3 CTAs per SM, of at most 1024

@@ -40,7 +40,8 @@
 // The running maximum is raised only when a score exceeds it by 2^8 (a vote
 // per group instead of shuffles and a rescale). Weights of an fp16 P carry 2^7
 // (paged_attn.cuh): rounding P to 16 bits is off by half a step of the operand
-// type relative to each weight, as in the framework's other attention kernels.
+// type relative to each weight, as in the framework's other tensor-core attention
+// kernels (the plain decode kernel, on the CUDA cores, keeps P in fp32).
 #include "paged_attn.cuh"
 #include "sm100.cuh"
 #include "tma_host.cuh"

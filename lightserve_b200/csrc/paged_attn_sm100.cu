@@ -14,7 +14,8 @@
 //    exist, or that no row sees, are fetched past the end: zeros.
 //  * e4m3 cache: TMA stages the raw tile, and a converter warpgroup multiplies
 //    each row by its power of two, rounds to q's type (exact in bf16, and in fp16
-//    within its range) and writes the swizzled tiles. (Two converter warpgroups
+//    for a cache written from fp16 rows; values below 2^-21 of one written from a
+//    wider type lose bits) and writes the swizzled tiles. (Two converter warpgroups
 //    took the registers of the softmax and were 12% slower; loading the raw
 //    rows into registers instead of staging them, 25%.)
 //  * V rows that no row of the item sees (past the context, between sinks and
@@ -30,7 +31,8 @@
 // the MMAs halve and the step stays. An e4m3 step is 17% longer: the converters
 // share shared memory and issue slots with the rest. Measured, 16 heads, one chunk
 // of 8192 tokens: D 128 bf16 222 us (1240 TFLOP/s), over e4m3 259; D 64 209 and 232.
-// (Tried: a share of the exponentials on the FMA pipe, +2 to +7%; an MMA warp per
+// (Tried: a share of the exponentials on the FMA pipe, D 128 +2% at an eighth to
+// +16% at a half, D 64 -2% to +22%; an MMA warp per
 // query tile, +25%, the tiles fall into step; three S buffers at D = 64, +8%;
 // six converter warps, +3 to +11%.)
 //

@@ -154,7 +154,8 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     values that no row of a sequence sees (past the context, before the window)
     are never used, whatever they hold; a NaN or infinity at a key that one row
     sees may reach the other new rows of its sequence. Sums are fp32 and
-    divided at the end: values times the number of keys stay below 2^119.
+    divided at the end: values times the number of keys stay below 2^119. Key
+    ranges are cut by the table's width: one much wider than its contexts is slower.
 
     Rows of q that belong to no sequence, or lie past ``max_seqlen_q`` of
     theirs, are not computed: their rows of ``out`` stay as they were. ``lse``
